@@ -152,6 +152,16 @@ int kth_copy(uint64_t dst, uint64_t dst_offset, uint64_t src, uint64_t src_offse
  * kth_release forgets it. */
 int kth_fill(uint64_t handle, uint64_t offset, uint64_t n, float value);
 
+/* The device address of a store's n_floats floats, for a host that shares the memory with another library of the same
+ * process and the same device (a tensor library that takes device pointers). No counterpart in the reference, whose
+ * stores are seen by their backend only. What the store was owed is launched first; from then on nothing about it is put
+ * off (fills, whole-store copies and small sums of and into it run at their call) and index values in it are checked at
+ * every use, so its memory always holds what the calls made so far say, in the order of the library's stream. The address
+ * stays valid until the store's last release. The library's stream knows nothing of the other library's work, nor that of
+ * this stream's: kth_sync before other code reads or writes the memory, and let that code's work finish before the next
+ * call that takes the store. n_floats may be NULL. */
+int kth_device_address(uint64_t handle, uint64_t* address, uint64_t* n_floats);
+
 /* containsNan (RAW:240, JVM:520-522). Blocking. */
 int kth_contains_nan(uint64_t handle, uint64_t n, int* out);
 
@@ -357,6 +367,49 @@ int kth_batch_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
 int kth_batch_norm_backward(uint64_t in, const int32_t* shape, int dims, int axis, int training, float epsilon,
                             uint64_t running_mean, uint64_t running_var, uint64_t current_mean, uint64_t current_std,
                             uint64_t gamma, uint64_t grad_out, uint64_t grad_in, uint64_t grad_gamma, uint64_t grad_beta);
+
+/* ------------------------------------------------------------------ layers over sequences */
+
+/* The operators of a residual block over sequences. The reference has none of them (its layers stop at batch
+ * normalisation); their operands follow kth_batch_norm_*: dense tensors of `shape`, `axis` already normalised, 0 for an
+ * operand that is not given or a result that is not required, sums and states in f64 inside. Deterministic. A result
+ * may share its store with another operand only where that is said. */
+
+/* Layer normalisation over the dims axis .. dims-1 (cols = their product, rows = that of the dims before):
+ * out = (in - mean) / sqrt(var + epsilon) * gamma + beta per row, var the mean squared deviation. gamma and beta hold
+ * cols floats or are 0 (1 and 0). current_mean and current_std (1 / sqrt(var + epsilon)) receive rows floats each or are
+ * 0. A row without variance gives beta, with epsilon 0 too. `out` may be `in`. epsilon < 0 or NaN: KTH_E_ARGUMENT. */
+int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis, float epsilon, uint64_t gamma, uint64_t beta,
+                           uint64_t out, uint64_t current_mean, uint64_t current_std);
+
+/* Its gradients from the forward call's operands (nothing else is saved; the rows' statistics are worked out again while
+ * the row is there): grad_in has `shape`, grad_gamma and grad_beta hold cols floats; each may be 0. grad_in may be grad_out. */
+int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axis, float epsilon, uint64_t gamma, uint64_t grad_out,
+                            uint64_t grad_in, uint64_t grad_gamma, uint64_t grad_beta);
+
+/* Dropout of n values: out[i] = r_i >= floor(p * 2^32) ? in[i] / (1 - p) : 0, plus residual[i] if one is given. The
+ * numbers r_i are words of the ten-round 4x32 counter-based generator of Salmon et al. (2011): key `seed`, counter
+ * offset + i / 4, word i % 4. Nothing is stored of them: the gradient is this call on the output's gradient with the same
+ * p, seed and offset. A layer that is called again advances its offset by (n + 3) / 4. A dropped value is 0 whatever it
+ * was (NaN and infinities too). `out` may be `in` or `residual`. p outside [0, 1]: KTH_E_ARGUMENT; p == 1 drops all. */
+int kth_dropout(uint64_t in, uint64_t n, double p, uint64_t seed, uint64_t offset, uint64_t residual, uint64_t out);
+
+/* How a gated recurrence takes its gate. */
+#define KTH_GATE_GIVEN   0    /* h_t = gate_t h_{t-1} + in_t */
+#define KTH_GATE_SIGMOID 1    /* h_t = s_t h_{t-1} + (1 - s_t) in_t, s = 1 / (1 + exp(-gate)) */
+
+/* The gated linear recurrence along `axis`, each position of the other dims (a channel) on its own: out_t = h_t, h_{-1} =
+ * initial (one float a channel, in the order of the other dims; 0: zeros); final_state receives the last step's state or
+ * is 0. One step at a time (shape[axis] == 1, initial and final_state the same store, which is then updated in place) is
+ * the form for single tokens. */
+int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial,
+                                 uint64_t out, uint64_t final_state);
+
+/* Its gradients. `out` is the forward call's result and `initial` the state it began with; grad_out the gradient of
+ * out, grad_final that of final_state (0: zeros). grad_gate, grad_in and grad_initial may each be 0. `in` is read in mode
+ * KTH_GATE_SIGMOID for grad_gate only, `out` and `initial` for grad_gate only: they may be 0 otherwise. */
+int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial, uint64_t out,
+                                  uint64_t grad_out, uint64_t grad_final, uint64_t grad_gate, uint64_t grad_in, uint64_t grad_initial);
 
 /* ------------------------------------------------------------------ control and metrics */
 

@@ -505,6 +505,8 @@ public:
         check(kth_read_scalar(storeReference, static_cast<uint64_t>(off), &v));
         return v;
     }
+    // The store's address on the device (kth_device_address), for another library of the process; valid until its last release.
+    uint64_t deviceAddress() { live(); uint64_t address = 0; check(kth_device_address(storeReference, &address, nullptr)); return address; }
     bool containsNan() { live(); int flag = 0; check(kth_contains_nan(storeReference, static_cast<uint64_t>(size()), &flag)); return flag != 0; }
     void inplaceFill(float value) { live(); check(kth_fill(storeReference, 0, static_cast<uint64_t>(size()), value)); }
     // inplaceResize (AbstractRawTensor.kt:242; JVMRawTensor.kt:524-531): a new store that keeps the

@@ -16,6 +16,7 @@ LIB_PATH = os.path.join(_HERE, "libkten_hip.so")
 
 KTH_MAX_DIMS = 10
 KTH_MATH_EXACT, KTH_MATH_WITHIN_2_ULP = 0, 1
+KTH_GATE_GIVEN, KTH_GATE_SIGMOID = 0, 1
 KTH_OK, KTH_E_NOT_INIT, KTH_E_HANDLE, KTH_E_ARGUMENT, KTH_E_SHAPE, KTH_E_MEMORY, KTH_E_DEVICE = 0, -1, -2, -3, -4, -5, -6
 
 
@@ -47,6 +48,7 @@ SIGNATURES = {
     "kth_read_scalar": (c_int, [c_uint64, c_uint64, POINTER(c_float)]),
     "kth_copy": (c_int, [c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
     "kth_fill": (c_int, [c_uint64, c_uint64, c_uint64, c_float]),
+    "kth_device_address": (c_int, [c_uint64, POINTER(c_uint64), POINTER(c_uint64)]),
     "kth_contains_nan": (c_int, [c_uint64, c_uint64, POINTER(c_int)]),
     "kth_binary": (c_int, [c_int, c_uint64, POINTER(c_int32), c_int, c_uint64, POINTER(c_int32), c_int,
                            c_uint64, POINTER(c_int32), c_int]),
@@ -77,6 +79,12 @@ SIGNATURES = {
                                        c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
     "kth_batch_norm_backward": (c_int, [c_uint64, POINTER(c_int32), c_int, c_int, c_int, c_float,
                                         c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
+    "kth_layer_norm_forward": (c_int, [c_uint64, POINTER(c_int32), c_int, c_int, c_float, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
+    "kth_layer_norm_backward": (c_int, [c_uint64, POINTER(c_int32), c_int, c_int, c_float, c_uint64, c_uint64, c_uint64, c_uint64, c_uint64]),
+    "kth_dropout": (c_int, [c_uint64, c_uint64, c_double, c_uint64, c_uint64, c_uint64, c_uint64]),
+    "kth_gated_recurrence_forward": (c_int, [c_uint64, c_uint64, POINTER(c_int32), c_int, c_int, c_int, c_uint64, c_uint64, c_uint64]),
+    "kth_gated_recurrence_backward": (c_int, [c_uint64, c_uint64, POINTER(c_int32), c_int, c_int, c_int, c_uint64, c_uint64, c_uint64,
+                                              c_uint64, c_uint64, c_uint64, c_uint64]),
     "kth_sync": (c_int, []),
     "kth_metrics": (c_int, [POINTER(c_uint64), POINTER(c_uint64), POINTER(c_uint64), POINTER(c_uint64)]),
 }

@@ -1186,7 +1186,8 @@ int kth_fill(uint64_t handle, uint64_t offset, uint64_t n, float value) {
         // A fill of the store's head is only noted: whoever reads the store next either folds the
         // constant into its own kernel or has the fill launched first (kth_internal.h, Store::fill_n).
         settle_for_overwrite(st, n);
-        st->fill_n = n; st->fill_value = value;
+        owe_fill(st, n, value);
+        KTH_LAUNCH_CHECK("fill");
         return KTH_OK;
     }
     settle(st);
@@ -1286,7 +1287,8 @@ int kth_scalar(int op, uint64_t a, float c, int reverse, uint64_t out, uint64_t 
     if (folds_a_constant(op) && sa->fill_n >= n && (so != sa || sa->fill_n == n) &&
         fold_constants(op, reverse ? c : sa->fill_value, reverse ? sa->fill_value : c, &folded)) {
         if (so != sa) settle_for_overwrite(so, n);
-        so->fill_n = n; so->fill_value = folded;
+        owe_fill(so, n, folded);
+        KTH_LAUNCH_CHECK("scalar");
         return KTH_OK;
     }
     settle(sa);
@@ -1296,6 +1298,7 @@ int kth_scalar(int op, uint64_t a, float c, int reverse, uint64_t out, uint64_t 
     // until one of the two stores is written
     if (op == KTH_POW && !rev && c == 1.0f && so != sa && n == so->n_floats) {
         make_alias(so, sa);
+        KTH_LAUNCH_CHECK("scalar");
         return KTH_OK;
     }
     const float* pa = sa->ptr; float* po = so->ptr; uint32_t n32 = static_cast<uint32_t>(n);
@@ -1470,7 +1473,8 @@ int kth_broadcast_to(uint64_t src, const int32_t* sshape, int sdims,
     if (ss != sd) settle_for_overwrite(sd, dn); else settle(sd);
     if (constant_source) {
         // every element of the result is the source's one constant: the result is owed the same fill
-        sd->fill_n = dn; sd->fill_value = ss->fill_value;
+        owe_fill(sd, dn, ss->fill_value);
+        KTH_LAUNCH_CHECK("broadcast_to");
         return KTH_OK;
     }
     if (sn == dn) {

@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -59,6 +60,10 @@ struct Store {
     // a write to the source launches the reduction first, like a copy that was put off. Whoever needs this store's
     // values gets them through `lookup`, which launches the reduction unless its caller asks for the note itself.
     struct OwedReduce { uint32_t src = 0; int op = 0; uint32_t outer = 0, axis = 0, inner = 0; } owed;
+    // Its address was handed out (kth_device_address): code outside the library may read and write its memory without a
+    // call that shows it, so nothing about the store is put off from then on (no owed fill, no alias in either direction,
+    // no owed reduction) and nothing is remembered of its values. `ptr` stays the same until the store is freed.
+    bool exported = false;
     uint32_t holds = 0;        // notes on other stores that need this one's values: it is freed when refs and holds are both 0
 };
 
@@ -160,10 +165,14 @@ int run_owed_reduce(int op, const float* in, float* out, uint32_t outer, uint32_
 void break_aliases(Store* st);
 // dst (no alias, no dependents, no owed fill: looked up for writing, and about to be overwritten whole) becomes a copy
 // of the first dst->n_floats values of src without a kernel. src holds at least as many values and is owed no fill.
+// (Where the address of one of the two is known outside the library the copy is made at once.)
 void make_alias(Store* dst, Store* src);
 // `lookup` for the index operand of an indexed move, which is only read: keeps the store's record of having been
 // checked as an index.
 Store* lookup_index(uint64_t handle, const char* what);
+// `st` (nothing owed) is to hold `value` in floats [0, n): noted, or launched at once if the store's address is known
+// outside the library.
+void owe_fill(Store* st, uint64_t n, float value);
 // Launches the fill the store is owed, if any, on the library's stream.
 void settle(Store* st);
 // The store is about to be written over floats [0, n) by a kernel that reads none of them: an owed
@@ -171,6 +180,19 @@ void settle(Store* st);
 void settle_for_overwrite(Store* st, uint64_t n);
 // fill_kernel over p[0, n) on the library's stream (kth_elementwise.hip).
 void launch_fill(float* p, uint64_t n, float value);
+
+// An operand of an entry point that takes many: `handle` 0 means that it is not given, otherwise its store must hold n floats.
+struct Operand {
+    const char* name;
+    uint64_t    handle, n;
+    bool        result;            // written whole in its first n floats (else only read)
+    Store*      store = nullptr;
+    float*      ptr = nullptr;     // set by resolve_operands; nullptr if not given
+};
+// Looks the operands up. Everything is checked before anything is launched: handles, sizes (size_code where a store is too
+// small), and that no result shares its store with another operand but for the `allowed` pairs (result, other). Then what
+// the inputs are owed is launched, and what the results are owed dropped or launched.
+int resolve_operands(const char* what, Operand* ops, int count, std::initializer_list<std::pair<int, int>> allowed, int size_code = KTH_E_SHAPE);
 
 // Pool-backed raw device memory for kernels' own workspaces (partials of two-pass
 // reductions). Stream-ordered: a workspace returned to the pool may be reused by a

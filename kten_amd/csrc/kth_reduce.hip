@@ -1091,7 +1091,7 @@ int reduce_axis_checked(const char* who, bool use_static, int op, uint64_t in, u
     // step, the two are one launch and this one's result is never written unless somebody else asks for it.
     {
         uint32_t groups, row_lanes;
-        if (!use_static && sums && i32 % 4 == 0 && i32 < 256 && outer * inner <= kSmallRowsFloats && si->alias_of == 0 &&
+        if (!use_static && sums && i32 % 4 == 0 && i32 < 256 && outer * inner <= kSmallRowsFloats && si->alias_of == 0 && !si->exported && !so->exported &&
             wave_slabs_plan(o32, a32, i32, &groups, &row_lanes)) {
             owe_reduce(so, si, op, o32, a32, i32);
             return KTH_OK;
@@ -1101,7 +1101,7 @@ int reduce_axis_checked(const char* who, bool use_static, int op, uint64_t in, u
                                    static_cast<uint32_t>(inner), use_static);
     // the positions ARG_MAX / ARG_MIN wrote are index values below the axis length: an indexed move that takes
     // them next (the scatter of a Max / Min backward) need not check them
-    if (rc == KTH_OK && (op == KTH_ARG_MAX || op == KTH_ARG_MIN)) {
+    if (rc == KTH_OK && (op == KTH_ARG_MAX || op == KTH_ARG_MIN) && !so->exported) {
         so->index_valid_below = static_cast<uint32_t>(axis);
         so->index_valid_n = outer * inner;
     }

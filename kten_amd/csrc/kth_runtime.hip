@@ -117,6 +117,7 @@ static void free_store(Store* st) {
 
 void make_alias(Store* dst, Store* src) {
     State& s = state();
+    if (dst->exported || src->exported) { launch_store_copy(src->ptr, dst->ptr, dst->n_floats); return; }
     if (src->alias_of != 0) src = &s.table[src->alias_of - 1];      // an alias of an alias is an alias of its source
     dst->own_ptr = dst->ptr;
     dst->ptr = src->ptr;
@@ -150,6 +151,11 @@ Store* lookup_unsettled(uint64_t handle, const char* what, bool only_reads, bool
     return &st;
 }
 
+void owe_fill(Store* st, uint64_t n, float value) {
+    if (st->exported) { launch_fill(st->ptr, n, value); return; }
+    st->fill_n = n; st->fill_value = value;
+}
+
 void settle(Store* st) {
     if (st->fill_n == 0) return;
     const uint64_t n = st->fill_n;
@@ -171,6 +177,37 @@ Store* lookup(uint64_t handle, const char* what, bool only_reads) {
 Store* lookup_index(uint64_t handle, const char* what) {
     // the index operand is only read: the store keeps what is known of it, and a copy it has put off stays put off
     return lookup(handle, what, true);
+}
+
+int resolve_operands(const char* what, Operand* ops, int count, std::initializer_list<std::pair<int, int>> allowed, int size_code) {
+    char label[96];
+    for (int i = 0; i < count; i++) {
+        Operand& o = ops[i];
+        if (o.handle == 0) continue;
+        snprintf(label, sizeof label, "%s(%s)", what, o.name);
+        o.store = lookup_unsettled(o.handle, label, true, true);       // (nothing is done to it yet)
+        if (!o.store) return KTH_E_HANDLE;
+        if (o.store->n_floats < o.n)
+            return fail(size_code, "%s holds %llu values, %llu are needed", label, (unsigned long long)o.store->n_floats, (unsigned long long)o.n);
+    }
+    for (int i = 0; i < count; i++)
+        for (int j = 0; j < count; j++) {
+            if (i == j || !ops[i].result || !ops[i].store || ops[i].store != ops[j].store) continue;
+            bool fine = false;
+            for (const std::pair<int, int>& p : allowed) fine = fine || (p.first == i && p.second == j);
+            if (!fine) return fail(KTH_E_ARGUMENT, "%s: %s and %s are the same store", what, ops[i].name, ops[j].name);
+        }
+    // results first: making the copies that were put off around them may move what the inputs read
+    for (int i = 0; i < count; i++)
+        if (ops[i].store && ops[i].result) (void)lookup_unsettled(ops[i].handle, what);
+    for (int i = 0; i < count; i++)
+        if (ops[i].store && !ops[i].result) (void)lookup(ops[i].handle, what, true);
+    for (int i = 0; i < count; i++) {
+        if (!ops[i].store) continue;
+        if (ops[i].result && ops[i].n != 0) settle_for_overwrite(ops[i].store, ops[i].n);      // (one that is an input too owes nothing any more)
+        ops[i].ptr = ops[i].store->ptr;
+    }
+    return KTH_OK;
 }
 
 // Size classes: 512-byte granules up to 1 MiB, then 1/8-octave steps (at most 12.5 %
@@ -426,7 +463,7 @@ int kth_alloc(uint64_t n_floats, uint64_t* handle) {
     else { idx = static_cast<uint32_t>(s.table.size()); s.table.emplace_back(); s.table.back().generation = g_epoch << 20; }
     Store& st = s.table[idx];
     st.ptr = p; st.n_floats = n_floats; st.cap_bytes = cap; st.refs = 1; st.fill_n = 0; st.index_valid_below = 0; st.index_valid_n = 0;
-    st.alias_of = 0; st.own_ptr = nullptr; st.dependents = 0; st.owed = Store::OwedReduce{}; st.holds = 0;
+    st.alias_of = 0; st.own_ptr = nullptr; st.dependents = 0; st.owed = Store::OwedReduce{}; st.holds = 0; st.exported = false;
     s.live_bytes += cap;
     *handle = make_handle(idx, st.generation);
     return KTH_OK;
@@ -477,7 +514,8 @@ int kth_upload(uint64_t handle, uint64_t offset, const float* src, uint64_t n) {
     if (n == 1 && offset == 0) {
         // One value (a [1]-shaped seed gradient, a scalar operand) is a fill of one float: noted, and
         // launched only if somebody reads the store as memory.
-        st->fill_n = 1; st->fill_value = src[0];
+        owe_fill(st, 1, src[0]);
+        KTH_LAUNCH_CHECK("kth_upload");
         return KTH_OK;
     }
     if (n <= kConstFloats) {
@@ -527,6 +565,19 @@ int kth_download(float* dst, uint64_t handle, uint64_t offset, uint64_t n) {
 int kth_read_scalar(uint64_t handle, uint64_t index, float* out) {
     if (!out) return fail(KTH_E_ARGUMENT, "kth_read_scalar: null output");
     return kth_download(out, handle, index, 1);
+}
+
+int kth_device_address(uint64_t handle, uint64_t* address, uint64_t* n_floats) {
+    std::lock_guard<std::mutex> g(lock());
+    KTH_REQUIRE_INIT();
+    if (!address) return fail(KTH_E_ARGUMENT, "kth_device_address: null address pointer");
+    Store* st = lookup(handle, "kth_device_address");
+    if (!st) return KTH_E_HANDLE;
+    KTH_LAUNCH_CHECK("kth_device_address");
+    st->exported = true;
+    *address = reinterpret_cast<uint64_t>(st->ptr);
+    if (n_floats) *n_floats = st->n_floats;
+    return KTH_OK;
 }
 
 namespace {
@@ -588,7 +639,8 @@ int kth_copy(uint64_t dst, uint64_t dst_offset, uint64_t src, uint64_t src_offse
     if (d != sst && dst_offset == 0 && sst->fill_n >= src_offset + n) {
         // a copy of floats that are all one owed constant: the head of the destination is owed it too
         settle_for_overwrite(d, n);
-        d->fill_n = n; d->fill_value = sst->fill_value;
+        owe_fill(d, n, sst->fill_value);
+        KTH_LAUNCH_CHECK("kth_copy");
         return KTH_OK;
     }
     settle(sst);
@@ -596,6 +648,7 @@ int kth_copy(uint64_t dst, uint64_t dst_offset, uint64_t src, uint64_t src_offse
     if (d != sst && dst_offset == 0 && src_offset == 0 && n == d->n_floats) {
         // the whole destination from the head of the source (copy(shallow = false)): put off until one of the two is written
         make_alias(d, sst);
+        KTH_LAUNCH_CHECK("kth_copy");
         return KTH_OK;
     }
     if (d->ptr == sst->ptr) {

@@ -350,6 +350,21 @@ class HipRawTensor(AbstractRawTensor):
         check(self.ops.lib.kth_download(host.ctypes.data_as(ctypes.c_void_p), self.storeReference, 0, self.size))
         return host.reshape(self.shape)
 
+    def deviceAddress(self) -> int:
+        """The address of the store's memory on the device (kth_device_address): valid until the store's last release.
+        The caller orders its own work with the library's stream (`ops.sync()` before it touches the memory)."""
+        self._require_live()
+        address = ctypes.c_uint64()
+        check(self.ops.lib.kth_device_address(self.storeReference, ctypes.byref(address), None))
+        return address.value
+
+    @property
+    def __cuda_array_interface__(self):
+        """The protocol by which array libraries take device memory without a copy: `torch.as_tensor(raw, device="cuda")`
+        is a tensor over the same memory and keeps this wrapper alive. The ordering is that of `deviceAddress`. A torch that
+        brings a HIP runtime of its own has to be imported before the first use of this package, so that both use that one."""
+        return {"shape": tuple(self.shape), "typestr": "<f4", "data": (self.deviceAddress(), False), "strides": None, "version": 2}
+
     def toList(self):
         return self.toArray().reshape(-1).tolist()
 
@@ -394,6 +409,131 @@ class HipBatchNorm:
             self.epsilon, self._h(runningMean), self._h(runningVar), self._h(currentMean), self._h(currentStd), self._h(gamma),
             gradOut.storeReference, self._h(gradIn), self._h(gradGamma), self._h(gradBeta)))
         return gradIn, gradGamma, gradBeta
+
+
+def _handle(t) -> int:
+    """The handle of an operand, 0 for one that is absent."""
+    if t is None:
+        return 0
+    t._require_live()
+    return t.storeReference
+
+
+def _require_size(what, t, n):
+    if t is not None and t.size != n:
+        raise ValueError(f"{what} must hold {n} values, got shape {t.shape}")
+
+
+class HipLayerNorm:
+    """Layer normalisation over the dims from `axis` on, shaped like `HipBatchNorm`. No counterpart in the reference."""
+
+    def __init__(self, axis, epsilon, ops):
+        self.axis, self.epsilon, self.ops = axis, float(epsilon), ops
+
+    def _rows_cols(self, input, gamma, beta):
+        axis = sf.normalize_axis(input.shape, self.axis)
+        cols = sf.to_store_size(input.shape[axis:])
+        _require_size("Gamma of a layer normalization", gamma, cols)
+        _require_size("Beta of a layer normalization", beta, cols)
+        return axis, input.shape[:axis] or [1], input.shape[axis:]
+
+    def calculateOutput(self, input, gamma=None, beta=None):
+        """(output, currentMean, currentStd = 1 / sqrt(var + epsilon)); the statistics have the shape of the dims before the axis."""
+        input._require_live()
+        axis, rows, _ = self._rows_cols(input, gamma, beta)
+        output, currentMean, currentStd = self.ops.createRaw(input.shape), self.ops.createRaw(rows), self.ops.createRaw(rows)
+        check(self.ops.lib.kth_layer_norm_forward(
+            input.storeReference, abi.shape_array(input.shape), input.dimensions, axis, self.epsilon, _handle(gamma), _handle(beta),
+            output.storeReference, currentMean.storeReference, currentStd.storeReference))
+        return output, currentMean, currentStd
+
+    def calculateGrads(self, input, gamma, gradOut, inRequiresGrad=True, gammaRequiresGrad=True, betaRequiresGrad=True):
+        if not (inRequiresGrad or gammaRequiresGrad or betaRequiresGrad):
+            return None, None, None
+        input._require_live(); gradOut._require_live()
+        axis, _, weights = self._rows_cols(input, gamma, None)
+        _require_size("The gradient of a layer normalization's output", gradOut, input.size)
+        gradIn = self.ops.createRaw(input.shape) if inRequiresGrad else None
+        gradGamma = self.ops.createRaw(weights) if gammaRequiresGrad else None
+        gradBeta = self.ops.createRaw(weights) if betaRequiresGrad else None
+        check(self.ops.lib.kth_layer_norm_backward(
+            input.storeReference, abi.shape_array(input.shape), input.dimensions, axis, self.epsilon, _handle(gamma),
+            gradOut.storeReference, _handle(gradIn), _handle(gradGamma), _handle(gradBeta)))
+        return gradIn, gradGamma, gradBeta
+
+
+class HipDropout:
+    """Dropout with the numbers of a counter-based generator (`kth_dropout`): p, seed and offset say which values are kept, so
+    the gradient needs nothing but the same call. No counterpart in the reference (its createBernoulli makes a mask tensor)."""
+
+    def __init__(self, p, seed, offset, ops):
+        self.p, self.seed, self.offset, self.ops = float(p), int(seed), int(offset), ops
+        if not 0.0 <= self.p <= 1.0:
+            raise ValueError(f"dropout probability {p} outside [0, 1]")
+        if not (0 <= self.seed < 1 << 64 and 0 <= self.offset < 1 << 64):
+            raise ValueError("seed and offset of a dropout are whole numbers below 2^64")
+
+    def calculateOutput(self, input, residual=None):
+        input._require_live()
+        _require_size("The residual of a dropout", residual, input.size)
+        output = self.ops.createRaw(input.shape)
+        check(self.ops.lib.kth_dropout(input.storeReference, input.size, self.p, self.seed, self.offset, _handle(residual), output.storeReference))
+        return output
+
+    def calculateGrad(self, gradOut):
+        """The gradient of the input; a residual's is gradOut itself."""
+        return self.calculateOutput(gradOut)
+
+
+class HipGatedRecurrence:
+    """h_t = a_t h_{t-1} + u_t along an axis (`kth_gated_recurrence_*`): with `sigmoidGate` a = sigmoid(gate) and u = (1 - a) input,
+    else a = gate and u = input. No counterpart in the reference."""
+
+    def __init__(self, axis, sigmoidGate, ops):
+        self.axis, self.ops = axis, ops
+        self.mode = abi.KTH_GATE_SIGMOID if sigmoidGate else abi.KTH_GATE_GIVEN
+
+    def _state_shape(self, gate, input, initial):
+        if gate.shape != input.shape:
+            raise ValueError(f"Gate and input of a recurrence must have the same shape, got {gate.shape} and {input.shape}")
+        axis = sf.normalize_axis(input.shape, self.axis)
+        state = input.shape[:axis] + input.shape[axis + 1:] or [1]
+        _require_size("The initial state of a recurrence", initial, sf.to_store_size(state))
+        return axis, state
+
+    def calculateOutput(self, gate, input, initial=None):
+        """(the states of all steps, the last step's state)."""
+        gate._require_live(); input._require_live()
+        axis, state = self._state_shape(gate, input, initial)
+        output, final = self.ops.createRaw(input.shape), self.ops.createRaw(state)
+        check(self.ops.lib.kth_gated_recurrence_forward(gate.storeReference, input.storeReference, abi.shape_array(input.shape), input.dimensions,
+                                                        axis, self.mode, _handle(initial), output.storeReference, final.storeReference))
+        return output, final
+
+    def step(self, gate, input, state):
+        """The states of the steps given (usually one), `state` being updated in place."""
+        gate._require_live(); input._require_live()
+        axis, _ = self._state_shape(gate, input, state)
+        output = self.ops.createRaw(input.shape)
+        check(self.ops.lib.kth_gated_recurrence_forward(gate.storeReference, input.storeReference, abi.shape_array(input.shape), input.dimensions,
+                                                        axis, self.mode, _handle(state), output.storeReference, _handle(state)))
+        return output
+
+    def calculateGrads(self, gate, input, initial, output, gradOut, gradFinal=None, gateRequiresGrad=True, inRequiresGrad=True, initialRequiresGrad=True):
+        if not (gateRequiresGrad or inRequiresGrad or initialRequiresGrad):
+            return None, None, None
+        gate._require_live(); gradOut._require_live()
+        axis, state = self._state_shape(gate, input, initial)
+        _require_size("The gradient of a recurrence's output", gradOut, gate.size)
+        _require_size("The output of a recurrence", output, gate.size)
+        _require_size("The gradient of a recurrence's last state", gradFinal, sf.to_store_size(state))
+        gradGate = self.ops.createRaw(gate.shape) if gateRequiresGrad else None
+        gradIn = self.ops.createRaw(gate.shape) if inRequiresGrad else None
+        gradInitial = self.ops.createRaw(state) if initialRequiresGrad else None
+        check(self.ops.lib.kth_gated_recurrence_backward(
+            gate.storeReference, _handle(input), abi.shape_array(gate.shape), gate.dimensions, axis, self.mode, _handle(initial), _handle(output),
+            gradOut.storeReference, _handle(gradFinal), _handle(gradGate), _handle(gradIn), _handle(gradInitial)))
+        return gradGate, gradIn, gradInitial
 
 
 class HipTensorOperations:
@@ -507,6 +647,15 @@ class HipTensorOperations:
     def batchNorm(self, axis: int, momentum: float, epsilon: float, training: bool) -> "HipBatchNorm":
         """TensorOperations.kt:129."""
         return HipBatchNorm(axis, momentum, epsilon, training, self)
+
+    def layerNorm(self, axis: int, epsilon: float) -> "HipLayerNorm":
+        return HipLayerNorm(axis, epsilon, self)
+
+    def dropout(self, p: float, seed: int, offset: int = 0) -> "HipDropout":
+        return HipDropout(p, seed, offset, self)
+
+    def gatedRecurrence(self, axis: int, sigmoidGate: bool = True) -> "HipGatedRecurrence":
+        return HipGatedRecurrence(axis, sigmoidGate, self)
 
     # --- Tensor-level factories (BasicTensorOperations.kt:10-12) ----------------------------
     def create(self, shape, requiresGrad: bool = False, init=None):

@@ -190,6 +190,21 @@ class AGTensor(Tensor):
         """functions/nn/TensorExtensions.kt: Tensor.batchNorm."""
         return BatchNormalizationFunction(axis, momentum, epsilon, training, self.ops)(self, runningMean, runningVar, gamma, beta)
 
+    def layerNorm(self, axis, epsilon=1e-5, gamma=None, beta=None):
+        """Layer normalisation over the dims from `axis` on."""
+        return LayerNormalizationFunction(axis, epsilon, self.ops)(self, gamma, beta)
+
+    def dropout(self, p, generator, training=True, residual=None):
+        """[residual +] dropout(this) with the next numbers of `generator`; outside training [residual +] this."""
+        if not training:
+            return self if residual is None else residual + self
+        return DropoutFunction(p, generator, self.ops)(self, residual)
+
+    def gatedRecurrence(self, axis, gate, initial=None, sigmoidGate=True):
+        """The states h_t = a_t h_{t-1} + u_t along `axis`; with `sigmoidGate` a = sigmoid(gate) and u = (1 - a) this, else
+        a = gate and u = this. The result's `finalState` is the last state, to go on from."""
+        return GatedRecurrenceFunction(axis, sigmoidGate, self.ops)(gate, self, initial)
+
     def meanVariance(self, axis, keepDimensions=False, unbiased=True):
         """AGTensor.kt:454-461."""
         tensor = _safe(self)
@@ -1382,6 +1397,164 @@ class BatchNormalizationFunction(Function):
             input, runningMean, runningVar, currentMean, currentStd, gamma, gradient,
             self.input.requiresGrad, self.gamma.requiresGrad if self.gamma is not None else False,
             self.beta.requiresGrad if self.beta is not None else False))
+
+
+class SequenceLayerFunction(Function):
+    """What the layers over sequences below share: several operands of which some may be absent (None), and one operand in
+    two places (an input that is its own residual), whose gradients are then added up before they are passed on."""
+
+    def __call__(self, *operands):
+        self.operands = [_safe(t) if t is not None else None for t in operands]
+        self.cachedShape = list(self.operands[0].shape)
+        return self
+
+    def getInputsAsList(self):
+        unique = []
+        for t in self.operands:
+            if t is not None and not any(t is u for u in unique):
+                unique.append(t)
+        return unique
+
+    def internalForward(self):
+        super().internalForward()
+        if self.hasValue():
+            return
+        fns = [t for t in self.getInputsAsList() if isinstance(t, Function)]
+        for f in fns:
+            f.internalForward()
+        if not self.hasValue():
+            self.doForward(*[None if t is None else t.getRawValue() for t in self.operands])
+        for f in fns:
+            f.mayFreeOutput()
+
+    def saveOperands(self, *raws):
+        """Keeps what the backward pass reads; absent ones stay in their places of `saved`."""
+        self.saved = raws
+        self.saveForBackward(*[r for r in raws if r is not None])
+
+    def doBackward(self, gradient):
+        if gradient.shape != self.cachedShape:
+            raise RuntimeError(f"Gradient shape mismatch, output grad shape: {gradient.shape} input shape: {self.cachedShape}")
+        grads = self.operandGradients(gradient, [t is not None and t.requiresGrad for t in self.operands])
+        result = []
+        for t in self.getInputsAsList():
+            own = [g for u, g in zip(self.operands, grads) if u is t and g is not None]
+            total = own[0] if own else None
+            for g in own[1:]:
+                total = total + g
+            result.append(total)
+        return result
+
+
+class LayerNormalizationFunction(SequenceLayerFunction):
+    """Layer normalisation as one raw call forward and one backward, shaped like BatchNormalizationFunction above; the
+    reference has none. Nothing but the input and gamma is saved."""
+
+    def __init__(self, axis, epsilon, ops):
+        super().__init__(ops)
+        self.axis, self.epsilon = axis, float(epsilon)
+
+    def __call__(self, input, gamma, beta):
+        super().__call__(input, gamma, beta)
+        axis = sf.normalize_axis(self.cachedShape, self.axis)
+        weights = self.cachedShape[axis:]
+        for t in self.operands[1:]:
+            if t is not None and list(t.shape) != weights:
+                raise ValueError(f"Gamma and beta parameters for layer normalization must have shape: {weights}, got {t.shape}")
+        self.layerNormOp = self.ops.layerNorm(axis, self.epsilon)
+        return self
+
+    def doForward(self, input, gamma, beta):
+        self.saveOperands(input, gamma)
+        self.output, mean, std = self.layerNormOp.calculateOutput(input, gamma, beta)
+        self.ops.release(mean, std)
+
+    def operandGradients(self, gradient, requires):
+        input, gamma = self.saved
+        return self.layerNormOp.calculateGrads(input, gamma, gradient, *requires)
+
+
+class CounterGenerator:
+    """Where a run's dropout layers take their numbers from: a seed and the next free counter. A layer reserves the counters
+    of its values when it is built, and its backward pass uses the same ones."""
+
+    def __init__(self, seed: int, offset: int = 0):
+        self.seed, self.offset = int(seed), int(offset)
+
+    def reserve(self, values: int) -> int:
+        """The first counter of `values` numbers, four to a counter (counters are 64 bits wide and wrap)."""
+        first = self.offset
+        self.offset = (first + (values + 3) // 4) % (1 << 64)
+        return first
+
+
+class DropoutFunction(SequenceLayerFunction):
+    """Dropout with the numbers of a CounterGenerator, plus a residual of the same shape if one is given. Nothing is saved."""
+
+    def __init__(self, p, generator, ops):
+        super().__init__(ops)
+        self.p, self.generator = float(p), generator
+
+    def __call__(self, input, residual):
+        super().__call__(input, residual)
+        if residual is not None and list(self.operands[1].shape) != self.cachedShape:
+            raise ValueError(f"The residual of a dropout must have its input's shape {self.cachedShape}, got {self.operands[1].shape}")
+        self.dropoutOp = self.ops.dropout(self.p, self.generator.seed, self.generator.offset)
+        self.generator.reserve(sf.to_store_size(self.cachedShape))
+        return self
+
+    def doForward(self, input, residual):
+        self.output = self.dropoutOp.calculateOutput(input, residual)
+
+    def operandGradients(self, gradient, requires):
+        return [self.dropoutOp.calculateGrad(gradient) if requires[0] else None, gradient.copy(shallow=True) if requires[1] else None]
+
+
+class GatedRecurrenceFunction(SequenceLayerFunction):
+    """The gated linear recurrence as one raw call forward and one backward. Gradients flow from the states, not from
+    `finalState`, which is what a next stretch of the same sequence starts from."""
+
+    def __init__(self, axis, sigmoidGate, ops):
+        super().__init__(ops)
+        self.axis, self.sigmoidGate = axis, bool(sigmoidGate)
+        self._final = None
+
+    def __call__(self, gate, input, initial):
+        super().__call__(gate, input, initial)
+        gate, input, initial = self.operands
+        if list(input.shape) != self.cachedShape:
+            raise ValueError(f"Gate and input of a recurrence must have the same shape, got {gate.shape} and {input.shape}")
+        axis = sf.normalize_axis(self.cachedShape, self.axis)
+        state = self.cachedShape[:axis] + self.cachedShape[axis + 1:] or [1]
+        if initial is not None and list(initial.shape) != state:
+            raise ValueError(f"The initial state of this recurrence must have shape {state}, got {initial.shape}")
+        self.recurrenceOp = self.ops.gatedRecurrence(axis, self.sigmoidGate)
+        return self
+
+    def doForward(self, gate, input, initial):
+        output, final = self.recurrenceOp.calculateOutput(gate, input, initial)
+        self._dropFinal()
+        self.ops.markSurviveGC(final)         # as long as this function is there, whatever scopes close meanwhile
+        self._final = final
+        self.saveOperands(gate, input, initial, output)
+        self.output = output
+
+    @property
+    def finalState(self):
+        if self._final is None:
+            self.forward()
+        return NoGradVariable(self.ops, self._final.copy(shallow=True))
+
+    def _dropFinal(self):
+        if self._final is not None:
+            self.ops.markReleasableInGC(self._final)       # the next scope that closes gives it back
+            self._final = None
+
+    def __del__(self):
+        self._dropFinal()
+
+    def operandGradients(self, gradient, requires):
+        return self.recurrenceOp.calculateGrads(*self.saved, gradient, None, *requires)
 
 
 class SoftmaxCrossEntropy(UnaryTensorFunction):
