@@ -28,28 +28,40 @@ struct ScanShape {
     FastDiv  inner_div;
 };
 
-// a and b = 1 - a of a gate, each to a relative error of a few 2^-24 (1 - a as a difference would lose it near a = 1,
-// and with it the decay over many steps).
+// exp(-|g|) to 2 u (u = 2^-24), results below the normal range included: 2^t by the hardware's exponential of t's fraction,
+// the rounding of t = -|g| log2(e) put back as a factor.
+__device__ __forceinline__ float exp_minus_abs(float g) {
+    const float x = fmaxf(-fabsf(g), -110.0f);               // (gives 0: below half the smallest float)
+    const float t = x * 1.44269504f;
+    const float low = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float n = rintf(t);
+    const float p = __builtin_amdgcn_exp2f(t - n);
+    return ldexpf(fmaf(p, low * 0.693147181f, p), static_cast<int>(n));
+}
+
+// 1 / d for d in [1, 2]: the hardware's reciprocal and a Newton step.
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+
+// A gate as the scans keep it in one register. GIVEN: the gate. SIGMOID: the smaller of a and 1 - a, with the sign of the
+// logit, which says which of the two it is: a and b = 1 - a then both come out to a few u of themselves (1 - a as a
+// difference from a rounded a would lose it near a = 1, and with it the decay over many steps).
 template <bool SIGMOID>
-struct Gate {
-    double a;
-    float  b;
-    __device__ __forceinline__ explicit Gate(float g) {
-        if (SIGMOID) {
-            const float e = expf(-fabsf(g));
-            const float r = 1.0f / (1.0f + e), s = e * r;
-            a = g >= 0.0f ? 1.0 - static_cast<double>(s) : static_cast<double>(s);
-            b = g >= 0.0f ? s : r;
-            if (g != g) { a = static_cast<double>(g); b = g; }
-        } else {
-            a = static_cast<double>(g);
-            b = 1.0f;
-        }
-    }
-    __device__ __forceinline__ double input(float x) const {
-        return SIGMOID ? static_cast<double>(b) * static_cast<double>(x) : static_cast<double>(x);
-    }
-};
+__device__ __forceinline__ float pack_gate(float g) {
+    if (!SIGMOID) return g;
+    const float e = exp_minus_abs(g);
+    const float m = copysignf(e * reciprocal(1.0f + e), g);
+    return g == g ? m : g;
+}
+template <bool SIGMOID>
+__device__ __forceinline__ double gate_a(float v) {
+    if (!SIGMOID) return static_cast<double>(v);
+    const double m = static_cast<double>(fabsf(v));
+    return __float_as_int(v) < 0 ? m : 1.0 - m;
+}
+__device__ __forceinline__ float sigmoid_b(float v) { return __float_as_int(v) < 0 ? 1.0f - fabsf(v) : fabsf(v); }
 
 // A thread per channel walks its steps.
 template <bool SIGMOID>
@@ -68,8 +80,8 @@ __global__ __launch_bounds__(kBlock) void recurrence_forward_kernel(const float*
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
             if (t0 + k < sh.steps) {
-                const Gate<SIGMOID> c(g[k]);
-                h = fma(c.a, h, c.input(x[k]));
+                const float v = pack_gate<SIGMOID>(g[k]);
+                h = fma(gate_a<SIGMOID>(v), h, static_cast<double>(SIGMOID ? sigmoid_b(v) * x[k] : x[k]));
                 out[at + static_cast<uint64_t>(k) * sh.inner] = static_cast<float>(h);
             }
         at += static_cast<uint64_t>(kAhead) * sh.inner;
@@ -91,20 +103,318 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
     for (uint32_t left = sh.steps; left > 0; left--) {
         const uint32_t t = left - 1;
         const uint64_t at = first + static_cast<uint64_t>(t) * sh.inner;
-        const Gate<SIGMOID> c(gate[at]);
+        const float v = pack_gate<SIGMOID>(gate[at]);
+        const double a = gate_a<SIGMOID>(v), b = SIGMOID ? static_cast<double>(sigmoid_b(v)) : 1.0;
         const double d = static_cast<double>(grad_out[at]) + carry;
         if (grad_gate) {                                 // (without it out and in need not be given)
             const float before = t > 0 ? out[at - sh.inner] : h0;
-            grad_gate[at] = static_cast<float>(SIGMOID ? d * (static_cast<double>(before) - static_cast<double>(in[at])) * (c.a * static_cast<double>(c.b))
+            grad_gate[at] = static_cast<float>(SIGMOID ? d * (static_cast<double>(before) - static_cast<double>(in[at])) * (a * b)
                                                        : d * static_cast<double>(before));
         }
-        if (grad_in) grad_in[at] = static_cast<float>(SIGMOID ? d * static_cast<double>(c.b) : d);
-        carry = c.a * d;
+        if (grad_in) grad_in[at] = static_cast<float>(d * b);
+        carry = a * d;
     }
     if (grad_initial) grad_initial[ch] = static_cast<float>(carry);
 }
 
+// ---------------------------------------------------------------- long sequences: tiles of steps
+
+// The scan is cut into tiles that pass a state on. A workgroup takes one tile: cw x 64 adjacent channels of one outer index
+// (a lane per channel) and tw x L successive steps, L to a wave, which the wave keeps in registers, so that every operand
+// is read once. A step is the map K -> a K + u of the state, so a run of steps is one pair (A, H): waves exchange theirs
+// through LDS, tiles through memory.
+//
+// Tiles are drawn by ticket, earliest steps of all channels first. A tile only waits for tiles of earlier steps, which
+// have lower tickets and thus run already or have ended: every wait ends. Tile p reads the pairs of the tiles since the
+// last multiple of kSuper before it, and the state that the tile before that multiple published: at most kSuper - 1 pairs
+// and one state, always composed in the same order, so the bits do not depend on who came first.
+//
+// A published value is one 64-bit word that carries its own sign of life, a double whose last kTagBits bits hold the
+// launch's number: no fence, no flag, no clearing between launches (the words are cleared when the number starts again).
+// What the doubles lose is 2^-41 of themselves a tile.
+constexpr int kTagBits = 12;
+constexpr uint32_t kTags = (1u << kTagBits) - 1;     // tag 0: never published
+constexpr uint32_t kSuper = 16;
+
+__device__ __forceinline__ void publish(uint64_t* word, double v, uint32_t tag) {
+    const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v)) + (1ull << (kTagBits - 1));
+    __hip_atomic_store(word, (bits & ~static_cast<uint64_t>(kTags)) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double await(const uint64_t* word, uint32_t tag) {
+    uint64_t bits = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    while ((bits & kTags) != tag) {
+        __builtin_amdgcn_s_sleep(1);
+        bits = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return __longlong_as_double(static_cast<long long>(bits & ~static_cast<uint64_t>(kTags)));
+}
+
+// A state that is zero stays so, whatever the product of the gates (which may have overflowed).
+__device__ __forceinline__ double advance(double A, double H, double state) { return state == 0.0 ? H : fma(A, state, H); }
+
+struct TilePlan {
+    uint32_t steps, inner;
+    uint32_t col_blocks, groups;     // workgroups across one outer index; across all channels (outer x col_blocks)
+    uint32_t tiles;                  // along the steps
+    uint32_t cw, tw;                 // waves of a workgroup across channels and along steps
+    uint32_t padded;                 // groups x cw x 64: channels with their padding
+    uint32_t tag;
+    uint32_t ticket_base;
+    uint32_t* tickets;
+    uint64_t* pairs;                 // [tiles][padded][2]
+    uint64_t* states;                // [tiles / kSuper][padded]
+    FastDiv  group_div, col_div;
+};
+
+struct Pair { double A, H; };
+
+// Keeps a value in its register as it is: what was worked out from it before is worked out again afterwards instead of
+// being kept too, which over a wave's steps would not fit the registers.
+__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+v"(v)); }
+// Keeps the instructions of few steps at a time in flight, for the same reason.
+#define KTH_STEPS_APART(k) do { if ((k) % 4 == 3) __builtin_amdgcn_sched_barrier(0); } while (0)
+
+// Where a workgroup and its waves stand.
+struct TilePlace {
+    uint32_t tile, group, lane, cwi, twi;
+    uint32_t channel;                // in its outer index
+    uint32_t slot;                   // among the padded channels
+    uint64_t base;                   // of the outer index's first step
+    uint32_t first_state;            // channel's place among all channels (outer x inner)
+    bool     valid;
+};
+
+__device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* lds_ticket) {
+    TilePlace w;
+    if (threadIdx.x == 0) *lds_ticket = pl.tiles > 1 ? atomicAdd(pl.tickets, 1u) - pl.ticket_base : blockIdx.x;
+    __syncthreads();
+    const uint32_t ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    w.lane = threadIdx.x & 63;
+    w.tile = divide(ticket, pl.group_div);
+    w.group = ticket - w.tile * pl.groups;
+    w.twi = wave / pl.cw;
+    w.cwi = wave - w.twi * pl.cw;
+    const uint32_t o = divide(w.group, pl.col_div);
+    const uint32_t c = ((w.group - o * pl.col_blocks) * pl.cw + w.cwi) * 64 + w.lane;
+    w.valid = c < pl.inner;
+    w.channel = w.valid ? c : pl.inner - 1;          // (a padding lane reads the last channel and writes nothing)
+    w.slot = (w.group * pl.cw + w.cwi) * 64 + w.lane;
+    w.base = static_cast<uint64_t>(o) * pl.steps * pl.inner;
+    w.first_state = o * pl.inner + w.channel;
+    return w;
+}
+
+// The state before this wave's first step, from the pair (A, H) of its steps. `initial` is the state before the first
+// tile. lds: pairs of the waves, [tw][cw * 64], then of the tiles before, as many again.
+__device__ __forceinline__ double state_before(const TilePlan& pl, const TilePlace& w, double A, double H, double initial, Pair* lds) {
+    const uint32_t width = pl.cw * 64, at = w.cwi * 64 + w.lane;
+    Pair* before = lds + pl.tw * width;
+    lds[w.twi * width + at] = Pair{A, H};
+    __syncthreads();
+    double state = initial;
+    const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
+    if (pl.tiles > 1) {
+        if (w.twi == pl.tw - 1 && w.tile + 1 < pl.tiles && many + 1 < kSuper) {
+            Pair total = lds[at];
+            for (uint32_t i = 1; i < pl.tw; i++) {
+                const Pair p = lds[i * width + at];
+                total = Pair{p.A * total.A, advance(p.A, p.H, total.H)};
+            }
+            if (w.tile == 0) total = Pair{0.0, advance(total.A, total.H, initial)};     // nobody else reads `initial`
+            uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
+            publish(word, total.A, pl.tag);
+            publish(word + 1, total.H, pl.tag);
+        }
+        if (w.tile > 0) {
+            // the waves along the steps share out the tiles before
+            const uint32_t per = (many + pl.tw - 1) / pl.tw;
+            const uint32_t from = min(w.twi * per, many), to = min(from + per, many);
+            Pair p{1.0, 0.0};
+            for (uint32_t i = from; i < to; i++) {
+                const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + i) * pl.padded + w.slot) * 2;
+                const double a = await(word, pl.tag), h = await(word + 1, pl.tag);
+                p = Pair{a * p.A, advance(a, h, p.H)};
+            }
+            before[w.twi * width + at] = p;
+            state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag);
+            __syncthreads();
+            for (uint32_t i = 0; i < pl.tw; i++) { const Pair q = before[i * width + at]; state = advance(q.A, q.H, state); }
+        }
+        if (w.twi == pl.tw - 1 && many + 1 == kSuper && w.tile + 1 < pl.tiles) {
+            double end = state;
+            for (uint32_t i = 0; i < pl.tw; i++) { const Pair q = lds[i * width + at]; end = advance(q.A, q.H, end); }
+            publish(pl.states + static_cast<uint64_t>(super) * pl.padded + w.slot, end, pl.tag);
+        }
+    }
+    for (uint32_t i = 0; i < w.twi; i++) { const Pair q = lds[i * width + at]; state = advance(q.A, q.H, state); }
+    return state;
+}
+
+constexpr uint32_t kTileThreads = 512;
+
+template <bool SIGMOID, int L>
+__global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kernel(const float* __restrict__ gate, const float* __restrict__ in, const float* initial,
+                                                                                   float* __restrict__ out, float* final_state, TilePlan pl) {
+    extern __shared__ Pair lds[];
+    __shared__ uint32_t lds_ticket;
+    const TilePlace w = place_tile(pl, &lds_ticket);
+    if (w.tile >= pl.tiles) return;
+    const uint32_t t0 = (w.tile * pl.tw + w.twi) * L;
+    const uint64_t row0 = w.base + static_cast<uint64_t>(t0) * pl.inner;
+    float v[L], u[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        const uint64_t row = w.base + static_cast<uint64_t>(min(t0 + k, pl.steps - 1)) * pl.inner;
+        v[k] = (gate + row)[w.channel];
+        u[k] = (in + row)[w.channel];
+    }
+#pragma unroll
+    for (int k = 0; k < L; k++)                              // a step behind the last one leaves the state as it is
+        if (t0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; u[k] = 0.0f; }
+    const double start = w.tile == 0 && initial ? static_cast<double>(initial[w.first_state]) : 0.0;
+    double A = 1.0, H = 0.0;
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        if (SIGMOID) {
+            v[k] = pack_gate<SIGMOID>(v[k]);
+            u[k] = sigmoid_b(v[k]) * u[k];
+        }
+        const double a = gate_a<SIGMOID>(v[k]);
+        H = fma(a, H, static_cast<double>(u[k]));
+        A *= a;
+        KTH_STEPS_APART(k);
+    }
+#pragma unroll
+    for (int k = 0; k < L; k++) { forget(v[k]); forget(u[k]); }
+    double h = state_before(pl, w, A, H, start, lds);
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        if (t0 + k < pl.steps) {
+            h = fma(gate_a<SIGMOID>(v[k]), h, static_cast<double>(u[k]));
+            if (w.valid) (out + row0 + static_cast<uint64_t>(k) * pl.inner)[w.channel] = static_cast<float>(h);
+        }
+        KTH_STEPS_APART(k);
+    }
+    if (final_state && w.valid && t0 < pl.steps && t0 + L >= pl.steps) final_state[w.first_state] = static_cast<float>(h);
+}
+
+// The gradient of the state runs from the last step to the first: K_t = a_t (grad_out_t + K_{t+1}), K behind the last step
+// being grad_final, d_t = grad_out_t + K_{t+1}; K_0 is grad_initial. Tiles, waves and steps are counted from the end.
+template <bool SIGMOID, int L>
+__global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_kernel(const float* __restrict__ gate, const float* __restrict__ in,
+                                                                                    const float* __restrict__ initial, const float* __restrict__ out,
+                                                                                    const float* __restrict__ grad_out, const float* __restrict__ grad_final,
+                                                                                    float* __restrict__ grad_gate, float* __restrict__ grad_in,
+                                                                                    float* __restrict__ grad_initial, TilePlan pl) {
+    extern __shared__ Pair lds[];
+    __shared__ uint32_t lds_ticket;
+    const TilePlace w = place_tile(pl, &lds_ticket);
+    if (w.tile >= pl.tiles) return;
+    const uint32_t q0 = (w.tile * pl.tw + w.twi) * L;        // step t = steps - 1 - (q0 + k)
+    const uint64_t last_row = w.base + static_cast<uint64_t>(pl.steps - 1) * pl.inner;
+    float v[L], g[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        const uint64_t row = last_row - static_cast<uint64_t>(min(q0 + k, pl.steps - 1)) * pl.inner;
+        v[k] = (gate + row)[w.channel];
+        g[k] = (grad_out + row)[w.channel];
+    }
+#pragma unroll
+    for (int k = 0; k < L; k++)
+        if (q0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; g[k] = 0.0f; }
+    const double start = w.tile == 0 && grad_final ? static_cast<double>(grad_final[w.first_state]) : 0.0;
+    double A = 1.0, H = 0.0;
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        if (SIGMOID) v[k] = pack_gate<SIGMOID>(v[k]);
+        const double a = gate_a<SIGMOID>(v[k]);
+        H = a * (static_cast<double>(g[k]) + H);
+        A *= a;
+        KTH_STEPS_APART(k);
+    }
+#pragma unroll
+    for (int k = 0; k < L; k++) { forget(v[k]); forget(g[k]); }
+    double K = state_before(pl, w, A, H, start, lds);
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        if (q0 + k < pl.steps) {
+            const uint64_t row = last_row - static_cast<uint64_t>(q0 + k) * pl.inner;
+            const double a = gate_a<SIGMOID>(v[k]), b = SIGMOID ? static_cast<double>(sigmoid_b(v[k])) : 1.0;
+            const double d = static_cast<double>(g[k]) + K;
+            if (grad_gate) {                                 // (without it out and in need not be given)
+                const float before = q0 + k + 1 < pl.steps ? (out + row - pl.inner)[w.channel] : initial ? initial[w.first_state] : 0.0f;
+                const double x = SIGMOID ? static_cast<double>((in + row)[w.channel]) : 0.0;
+                const double r = SIGMOID ? d * (static_cast<double>(before) - x) * (a * b) : d * static_cast<double>(before);
+                if (w.valid) (grad_gate + row)[w.channel] = static_cast<float>(r);
+            }
+            if (grad_in && w.valid) (grad_in + row)[w.channel] = static_cast<float>(d * b);
+            K = a * d;
+        }
+        KTH_STEPS_APART(k);
+    }
+    if (grad_initial && w.valid && q0 < pl.steps && q0 + L >= pl.steps) grad_initial[w.first_state] = static_cast<float>(K);
+}
+
 // ---------------------------------------------------------------- host side
+
+// Up to here a thread walks all steps of its channel.
+constexpr uint32_t kShortSteps = 32;
+
+// The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
+// one stream, and each has a tag and a range of tickets of its own.
+int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
+    TilePlan pl{};
+    pl.steps = sh.steps; pl.inner = sh.inner;
+    pl.cw = 1; pl.tw = kTileThreads / 64;
+    pl.col_blocks = (sh.inner + pl.cw * 64 - 1) / (pl.cw * 64);
+    pl.groups = sh.outer * pl.col_blocks;
+    pl.tiles = (sh.steps + pl.tw * L - 1) / (pl.tw * L);
+    pl.padded = pl.groups * pl.cw * 64;
+    pl.group_div = make_div(pl.groups);
+    pl.col_div = make_div(pl.col_blocks);
+    if (pl.tiles > 1) {
+        State& s = state();
+        const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.padded * 2;
+        const uint64_t words = 64 + pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded;
+        if (words > s.scan_words || s.scan_tag == kTags) {
+            if (words > s.scan_words) {
+                KTH_HIP(hipStreamSynchronize(s.stream));
+                if (s.scan) KTH_HIP(hipFree(s.scan));
+                s.scan = nullptr; s.scan_words = 0;
+                void* p = nullptr;
+                if (hipMalloc(&p, words * 8) != hipSuccess) {
+                    (void)hipGetLastError();
+                    return fail(KTH_E_MEMORY, "%s: no workspace of %llu bytes", what, static_cast<unsigned long long>(words * 8));
+                }
+                s.scan = static_cast<uint64_t*>(p);
+                s.scan_words = words;
+            }
+            for (uint64_t at = 0; at < s.scan_words; at += 1ull << 29)
+                launch_fill(reinterpret_cast<float*>(s.scan + at), 2 * std::min<uint64_t>(s.scan_words - at, 1ull << 29), 0.0f);
+            s.scan_tag = 0; s.scan_tickets = 0;
+        }
+        s.scan_tag += 1;
+        pl.tag = s.scan_tag;
+        pl.ticket_base = s.scan_tickets;
+        s.scan_tickets += pl.tiles * pl.groups;              // (wraps, as the counter does)
+        pl.tickets = reinterpret_cast<uint32_t*>(s.scan);
+        pl.pairs = s.scan + 64;
+        pl.states = pl.pairs + pairs;
+    }
+    *out = pl;
+    return KTH_OK;
+}
+
+// A launch that failed drew no tickets: the next one starts from cleared words.
+int tiles_launched(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return KTH_OK;
+    state().scan_tag = kTags;
+    return fail(KTH_E_DEVICE, "launch of %s failed: %s", what, hipGetErrorString(e));
+}
+
+uint32_t tile_lds(const TilePlan& pl) { return 2 * pl.tw * pl.cw * 64 * static_cast<uint32_t>(sizeof(Pair)); }
 
 int shape_of(const char* what, const int32_t* shape, int dims, int axis, int mode, ScanShape* sh, uint64_t* n) {
     if (mode != KTH_GATE_GIVEN && mode != KTH_GATE_SIGMOID) return fail(KTH_E_ARGUMENT, "%s: gate mode %d", what, mode);
@@ -143,9 +453,20 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
     Operand ops[5] = {{"gate", gate, n, false}, {"in", in, n, false}, {"initial", initial, sh.channels, false},
                       {"out", out, n, true}, {"final_state", final_state, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 5, {{4, 2}})) return rc;          // the state may be updated in place
-    LaunchScope scope("recurrence_forward_kernel", mode == KTH_GATE_SIGMOID ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
+    const bool sigmoid = mode == KTH_GATE_SIGMOID;
+    if (sh.steps > kShortSteps && sh.inner >= 32) {
+        constexpr int L = 32;
+        TilePlan pl;
+        if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
+        LaunchScope scope("recurrence_forward_tiles_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
+        const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
+        if (sigmoid) hipLaunchKernelGGL((recurrence_forward_tiles_kernel<true, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
+        else         hipLaunchKernelGGL((recurrence_forward_tiles_kernel<false, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
+        return tiles_launched("gated_recurrence_forward");
+    }
+    LaunchScope scope("recurrence_forward_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);
-    if (mode == KTH_GATE_SIGMOID)
+    if (sigmoid)
         hipLaunchKernelGGL((recurrence_forward_kernel<true>), grid, dim3(kBlock), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, sh);
     else
         hipLaunchKernelGGL((recurrence_forward_kernel<false>), grid, dim3(kBlock), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, sh);
@@ -171,6 +492,18 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                       {"grad_gate", grad_gate, n, true}, {"grad_in", grad_in, n, true},
                       {"grad_initial", grad_initial, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 9, {})) return rc;
+    if (sh.steps > kShortSteps && sh.inner >= 32) {
+        constexpr int L = 16;
+        TilePlan pl;
+        if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
+        LaunchScope scope("recurrence_backward_tiles_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
+        const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
+        if (sigmoid) hipLaunchKernelGGL((recurrence_backward_tiles_kernel<true, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
+                                        ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
+        else         hipLaunchKernelGGL((recurrence_backward_tiles_kernel<false, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
+                                        ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
+        return tiles_launched("gated_recurrence_backward");
+    }
     LaunchScope scope("recurrence_backward_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);
     if (sigmoid)

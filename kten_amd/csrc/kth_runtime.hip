@@ -348,6 +348,7 @@ static void teardown() {
     s.free_slots.clear();
     trim_pool();
     if (s.deferred_index_flag) (void)hipFree(s.deferred_index_flag);
+    if (s.scan) (void)hipFree(s.scan);
     if (s.host_index_flag) (void)hipHostFree(const_cast<int*>(s.host_index_flag));
     s.host_index_flag = nullptr; s.host_index_flag_device = nullptr;
     for (LaunchRecord& r : s.records) { (void)hipEventDestroy(r.begin); (void)hipEventDestroy(r.end); }
