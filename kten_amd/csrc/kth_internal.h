@@ -285,6 +285,10 @@ inline void launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t ld
             return kth::fail(KTH_E_DEVICE, "launch of %s failed: %s", name, hipGetErrorString(e__)); \
     } while (0)
 
+// Keeps a value in its register as it is: what was worked out from it before (its f64 copy) is worked out again afterwards
+// instead of being kept too, where a lane holds many values and both would not fit its registers.
+__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+v"(v)); }
+
 constexpr uint64_t kMaxElements = 0x7fffffffull;   // store size is a Kotlin Int
 
 }  // namespace kth

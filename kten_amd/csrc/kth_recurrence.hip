@@ -28,15 +28,14 @@ struct ScanShape {
     FastDiv  inner_div;
 };
 
-// exp(-|g|) to 2 u (u = 2^-24), results below the normal range included: 2^t by the hardware's exponential of t's fraction,
-// the rounding of t = -|g| log2(e) put back as a factor.
+// exp(-|g|) to 2 u (u = 2^-24), results below the normal range included: 2^(f + n) with f the fraction of |g| log2(e), in
+// two products, by the hardware's exponential.
 __device__ __forceinline__ float exp_minus_abs(float g) {
-    const float x = fmaxf(-fabsf(g), -110.0f);               // (gives 0: below half the smallest float)
-    const float t = x * 1.44269504f;
-    const float low = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-    const float n = rintf(t);
-    const float p = __builtin_amdgcn_exp2f(t - n);
-    return ldexpf(fmaf(p, low * 0.693147181f, p), static_cast<int>(n));
+    float x = -fabsf(g);
+    x = x < -110.0f ? -110.0f : x;                           // (gives 0: below half the smallest float; NaN stays NaN)
+    const float n = rintf(x * 1.44269504f);
+    const float f = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -n));
+    return ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
 }
 
 // 1 / d for d in [1, 2]: the hardware's reciprocal and a Newton step.
@@ -45,23 +44,24 @@ __device__ __forceinline__ float reciprocal(float d) {
     return fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 
-// A gate as the scans keep it in one register. GIVEN: the gate. SIGMOID: the smaller of a and 1 - a, with the sign of the
-// logit, which says which of the two it is: a and b = 1 - a then both come out to a few u of themselves (1 - a as a
-// difference from a rounded a would lose it near a = 1, and with it the decay over many steps).
+// A gate as the scans keep it in one register. GIVEN: the gate. SIGMOID: s, the smaller of a and b = 1 - a, with the sign of
+// the logit, which says which of the two it is: a = 1 - s or 0 + s, b = 0 + s or 1 - s. Both come out to a few u of
+// themselves (b as a difference from a rounded a would be lost near a = 1, and with it the decay over many steps).
 template <bool SIGMOID>
 __device__ __forceinline__ float pack_gate(float g) {
     if (!SIGMOID) return g;
     const float e = exp_minus_abs(g);
-    const float m = copysignf(e * reciprocal(1.0f + e), g);
-    return g == g ? m : g;
+    return copysignf(e * reciprocal(1.0f + e), g);
 }
 template <bool SIGMOID>
 __device__ __forceinline__ double gate_a(float v) {
     if (!SIGMOID) return static_cast<double>(v);
-    const double m = static_cast<double>(fabsf(v));
-    return __float_as_int(v) < 0 ? m : 1.0 - m;
+    const int one = ~(__float_as_int(v) >> 31) & 0x3ff00000;             // the high word of 1.0 or 0.0
+    return __hiloint2double(one, 0) - static_cast<double>(v);
 }
-__device__ __forceinline__ float sigmoid_b(float v) { return __float_as_int(v) < 0 ? 1.0f - fabsf(v) : fabsf(v); }
+__device__ __forceinline__ float sigmoid_b(float v) {
+    return __int_as_float((__float_as_int(v) >> 31) & 0x3f800000) + v;   // 1 or 0
+}
 
 // A thread per channel walks its steps.
 template <bool SIGMOID>
@@ -168,9 +168,6 @@ struct TilePlan {
 
 struct Pair { double A, H; };
 
-// Keeps a value in its register as it is: what was worked out from it before is worked out again afterwards instead of
-// being kept too, which over a wave's steps would not fit the registers.
-__device__ __forceinline__ void forget(float& v) { asm volatile("" : "+v"(v)); }
 // Keeps the instructions of few steps at a time in flight, for the same reason.
 #define KTH_STEPS_APART(k) do { if ((k) % 4 == 3) __builtin_amdgcn_sched_barrier(0); } while (0)
 
@@ -253,7 +250,12 @@ __device__ __forceinline__ double state_before(const TilePlan& pl, const TilePla
 
 constexpr uint32_t kTileThreads = 512;
 
-template <bool SIGMOID, int L>
+// LINES: rows are multiples of 128 bytes, so no two workgroups read the same cache line and it need not be kept
+// ([8,2048,1024] 53 to 50 us; with odd rows the lines' second readers would wait: [5,1999,1001] backward 70 to 75 us).
+template <bool LINES>
+__device__ __forceinline__ float read_once(const float* p) { return LINES ? __builtin_nontemporal_load(p) : *p; }
+
+template <bool SIGMOID, bool LINES, int L>
 __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kernel(const float* __restrict__ gate, const float* __restrict__ in, const float* initial,
                                                                                    float* __restrict__ out, float* final_state, TilePlan pl) {
     extern __shared__ Pair lds[];
@@ -266,8 +268,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
 #pragma unroll
     for (int k = 0; k < L; k++) {
         const uint64_t row = w.base + static_cast<uint64_t>(min(t0 + k, pl.steps - 1)) * pl.inner;
-        v[k] = (gate + row)[w.channel];
-        u[k] = (in + row)[w.channel];
+        v[k] = read_once<LINES>(gate + row + w.channel);
+        u[k] = read_once<LINES>(in + row + w.channel);
     }
 #pragma unroll
     for (int k = 0; k < L; k++)                              // a step behind the last one leaves the state as it is
@@ -301,7 +303,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
 
 // The gradient of the state runs from the last step to the first: K_t = a_t (grad_out_t + K_{t+1}), K behind the last step
 // being grad_final, d_t = grad_out_t + K_{t+1}; K_0 is grad_initial. Tiles, waves and steps are counted from the end.
-template <bool SIGMOID, int L>
+template <bool SIGMOID, bool LINES, int L>
 __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_kernel(const float* __restrict__ gate, const float* __restrict__ in,
                                                                                     const float* __restrict__ initial, const float* __restrict__ out,
                                                                                     const float* __restrict__ grad_out, const float* __restrict__ grad_final,
@@ -317,8 +319,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
 #pragma unroll
     for (int k = 0; k < L; k++) {
         const uint64_t row = last_row - static_cast<uint64_t>(min(q0 + k, pl.steps - 1)) * pl.inner;
-        v[k] = (gate + row)[w.channel];
-        g[k] = (grad_out + row)[w.channel];
+        v[k] = read_once<LINES>(gate + row + w.channel);
+        g[k] = read_once<LINES>(grad_out + row + w.channel);
     }
 #pragma unroll
     for (int k = 0; k < L; k++)
@@ -335,6 +337,22 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
     }
 #pragma unroll
     for (int k = 0; k < L; k++) { forget(v[k]); forget(g[k]); }
+    // what only the gate's gradient needs arrives while the state does (without it out and in need not be given)
+    float before[L], x[L];
+    if (grad_gate) {
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            const uint32_t q = min(q0 + k, pl.steps - 1);
+            const uint64_t row = last_row - static_cast<uint64_t>(q) * pl.inner;
+            before[k] = (out + (q + 1 < pl.steps ? row - pl.inner : row))[w.channel];
+            if (SIGMOID) x[k] = read_once<LINES>(in + row + w.channel);
+        }
+        if (q0 < pl.steps && q0 + L >= pl.steps) {
+            const float h0 = initial ? initial[w.first_state] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < L; k++) if (q0 + k + 1 == pl.steps) before[k] = h0;
+        }
+    }
     double K = state_before(pl, w, A, H, start, lds);
 #pragma unroll
     for (int k = 0; k < L; k++) {
@@ -342,10 +360,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
             const uint64_t row = last_row - static_cast<uint64_t>(q0 + k) * pl.inner;
             const double a = gate_a<SIGMOID>(v[k]), b = SIGMOID ? static_cast<double>(sigmoid_b(v[k])) : 1.0;
             const double d = static_cast<double>(g[k]) + K;
-            if (grad_gate) {                                 // (without it out and in need not be given)
-                const float before = q0 + k + 1 < pl.steps ? (out + row - pl.inner)[w.channel] : initial ? initial[w.first_state] : 0.0f;
-                const double x = SIGMOID ? static_cast<double>((in + row)[w.channel]) : 0.0;
-                const double r = SIGMOID ? d * (static_cast<double>(before) - x) * (a * b) : d * static_cast<double>(before);
+            if (grad_gate) {
+                const double r = SIGMOID ? d * (static_cast<double>(before[k]) - static_cast<double>(x[k])) * (a * b) : d * static_cast<double>(before[k]);
                 if (w.valid) (grad_gate + row)[w.channel] = static_cast<float>(r);
             }
             if (grad_in && w.valid) (grad_in + row)[w.channel] = static_cast<float>(d * b);
@@ -359,14 +375,14 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
 // ---------------------------------------------------------------- host side
 
 // Up to here a thread walks all steps of its channel.
-constexpr uint32_t kShortSteps = 32;
+constexpr uint32_t kShortForward = 32, kShortBackward = 4;
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
 // one stream, and each has a tag and a range of tickets of its own.
 int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     TilePlan pl{};
     pl.steps = sh.steps; pl.inner = sh.inner;
-    pl.cw = 1; pl.tw = kTileThreads / 64;
+    pl.cw = 1; pl.tw = std::min<uint32_t>(kTileThreads / 64, (sh.steps + L - 1) / L);
     pl.col_blocks = (sh.inner + pl.cw * 64 - 1) / (pl.cw * 64);
     pl.groups = sh.outer * pl.col_blocks;
     pl.tiles = (sh.steps + pl.tw * L - 1) / (pl.tw * L);
@@ -454,14 +470,16 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
                       {"out", out, n, true}, {"final_state", final_state, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 5, {{4, 2}})) return rc;          // the state may be updated in place
     const bool sigmoid = mode == KTH_GATE_SIGMOID;
-    if (sh.steps > kShortSteps && sh.inner >= 32) {
+    if (sh.steps > kShortForward && sh.inner >= 32) {
         constexpr int L = 32;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
         LaunchScope scope("recurrence_forward_tiles_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
         const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
-        if (sigmoid) hipLaunchKernelGGL((recurrence_forward_tiles_kernel<true, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
-        else         hipLaunchKernelGGL((recurrence_forward_tiles_kernel<false, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
+        const bool lines = sh.inner % 32 == 0;
+        auto* kernel = sigmoid ? (lines ? recurrence_forward_tiles_kernel<true, true, L> : recurrence_forward_tiles_kernel<true, false, L>)
+                               : (lines ? recurrence_forward_tiles_kernel<false, true, L> : recurrence_forward_tiles_kernel<false, false, L>);
+        hipLaunchKernelGGL(kernel, grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
         return tiles_launched("gated_recurrence_forward");
     }
     LaunchScope scope("recurrence_forward_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
@@ -492,16 +510,17 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                       {"grad_gate", grad_gate, n, true}, {"grad_in", grad_in, n, true},
                       {"grad_initial", grad_initial, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 9, {})) return rc;
-    if (sh.steps > kShortSteps && sh.inner >= 32) {
+    if (sh.steps > kShortBackward && sh.inner >= 32) {
         constexpr int L = 16;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
         LaunchScope scope("recurrence_backward_tiles_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
         const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
-        if (sigmoid) hipLaunchKernelGGL((recurrence_backward_tiles_kernel<true, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
-                                        ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
-        else         hipLaunchKernelGGL((recurrence_backward_tiles_kernel<false, L>), grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
-                                        ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
+        const bool lines = sh.inner % 32 == 0;
+        auto* kernel = sigmoid ? (lines ? recurrence_backward_tiles_kernel<true, true, L> : recurrence_backward_tiles_kernel<true, false, L>)
+                               : (lines ? recurrence_backward_tiles_kernel<false, true, L> : recurrence_backward_tiles_kernel<false, false, L>);
+        hipLaunchKernelGGL(kernel, grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
+                           ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
         return tiles_launched("gated_recurrence_backward");
     }
     LaunchScope scope("recurrence_backward_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
