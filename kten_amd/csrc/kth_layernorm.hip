@@ -69,6 +69,207 @@ __device__ __forceinline__ void block_fold(double (&s)[NS], double* lds) {
     }
 }
 
+// ---------------------------------------------------------------- rows that stay in registers
+
+// G lanes hold a row, U float4s each (column (u G + lane) 4 + e), so that a pass reads its operands once: a row is summed,
+// its statistics are worked out by every lane, and the results are written from the registers. G = 4, 16 and 64 put
+// several rows into a wave or one, larger G a row into a workgroup; a grid that fills the chip strides over the rows and
+// keeps the weights.
+template <int G>
+struct RowGroup {
+    static constexpr int threads = G > kBlock ? G : kBlock;
+    static constexpr int groups = threads / G;                 // rows of a workgroup at a time
+    static constexpr int waves = G > 64 ? G / 64 : 0;          // that share a row
+};
+
+// Sums of NS doubles over the G lanes of a row; every lane gets them, added in the same order. `lds` holds two sets of
+// NS x waves doubles: sets alternate from row to row, so one barrier a row is enough.
+template <int G, int NS>
+__device__ __forceinline__ void row_fold(double (&s)[NS], double* lds, uint32_t& set) {
+#pragma unroll
+    for (int off = (G > 64 ? 64 : G) / 2; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < NS; i++) s[i] += __shfl_xor(s[i], off);
+    if constexpr (G > 64) {
+        constexpr int waves = RowGroup<G>::waves;
+        double* mine = lds + set * NS * waves;
+        set ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < NS; i++) mine[i * waves + (threadIdx.x >> 6)] = s[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            s[i] = mine[i * waves];
+#pragma unroll
+            for (int w = 1; w < waves; w++) s[i] += mine[i * waves + w];
+        }
+    }
+}
+
+// 1 / sqrt(v + eps) in f64: the hardware's estimate (24 bits) and one Newton step.
+__device__ __forceinline__ double row_rstd_fast(double v, double eps) {
+    const double s = v + eps;
+    if (s == 0.0) return 0.0;
+    const double y = __builtin_amdgcn_rsq(s);
+    return fma(0.5 * y, fma(-s * y, y, 1.0), y);
+}
+
+// Four values from column c on; `fill` behind the last column.
+template <bool ONCE>
+__device__ __forceinline__ void load4(const float* p, uint32_t c, uint32_t cols, float fill, float (&v)[4]) {
+    if (c + 4 <= cols) {
+        const v4f_any* q = reinterpret_cast<const v4f_any*>(p + c);
+        const v4f_any t = ONCE ? __builtin_nontemporal_load(q) : *q;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = t[e];
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) v[e] = c + e < cols ? p[c + e] : fill;
+    }
+}
+__device__ __forceinline__ void store4(float* p, uint32_t c, uint32_t cols, const float (&v)[4]) {
+    if (c + 4 <= cols) {
+        *reinterpret_cast<v4f_any*>(p + c) = v4f_any{v[0], v[1], v[2], v[3]};
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) if (c + e < cols) p[c + e] = v[e];
+    }
+}
+
+template <int G, int U>
+__global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                               float* out, float* __restrict__ out_mean, float* __restrict__ out_std,
+                                                                               Shape2 sh, double eps) {
+    __shared__ double lds[G > 64 ? 2 * 2 * RowGroup<G>::waves : 1];
+    const uint32_t lane = threadIdx.x % G;
+    uint32_t set = 0;
+    float ga[U][4], be[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t c = (u * G + lane) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++) { ga[u][e] = 1.0f; be[u][e] = 0.0f; }
+        if (gamma) load4<false>(gamma, c, sh.cols, 1.0f, ga[u]);
+        if (beta) load4<false>(beta, c, sh.cols, 0.0f, be[u]);
+    }
+    for (uint32_t row = blockIdx.x * RowGroup<G>::groups + threadIdx.x / G; row < sh.rows; row += gridDim.x * RowGroup<G>::groups) {
+        const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
+        const float first = x[at];
+        float v[U][4];
+#pragma unroll
+        for (int u = 0; u < U; u++) load4<true>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
+        const double k = static_cast<double>(first);
+        double s[2] = {};
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) { const double d = static_cast<double>(v[u][e]) - k; s[0] += d; s[1] = fma(d, d, s[1]); }
+        row_fold<G, 2>(s, lds, set);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) forget(v[u][e]);
+        const double mean = k + s[0] * sh.inv_cols;
+        const float rstd = static_cast<float>(row_rstd_fast(row_variance(s[0], s[1], sh.inv_cols), eps));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float r[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] = ln_forward(v[u][e], mean, rstd, ga[u][e], be[u][e]);
+            store4(out + at, (u * G + lane) * 4, sh.cols, r);
+        }
+        if (lane == 0) {
+            if (out_mean) out_mean[row] = static_cast<float>(mean);
+            if (out_std) out_std[row] = rstd;
+        }
+    }
+}
+
+// The input gradient of each row, and down the workgroup's rows the weights' gradients, in f64 registers; a workgroup
+// leaves one row [2, cols] of partial sums as floats, each rounded once (2^-24 of itself), which ln_fold_kernel adds in f64.
+template <int G, int U>
+__global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
+                                                                                float* __restrict__ partial, Shape2 sh, double eps) {
+    constexpr int threads = RowGroup<G>::threads, groups = RowGroup<G>::groups;
+    __shared__ double lds[G > 64 ? 2 * 4 * RowGroup<G>::waves : threads * 4];
+    const uint32_t lane = threadIdx.x % G;
+    uint32_t set = 0;
+    float ga[U][4];
+    double sg[U][4], sb[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) { ga[u][e] = 1.0f; sg[u][e] = 0.0; sb[u][e] = 0.0; }
+        if (gamma) load4<false>(gamma, (u * G + lane) * 4, sh.cols, 1.0f, ga[u]);
+    }
+    for (uint32_t row = blockIdx.x * groups + threadIdx.x / G; row < sh.rows; row += gridDim.x * groups) {
+        const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
+        const float first = x[at];
+        float v[U][4], g[U][4];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            load4<true>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
+            load4<true>(go + at, (u * G + lane) * 4, sh.cols, 0.0f, g[u]);
+        }
+        const double k = static_cast<double>(first);
+        double s[4] = {};
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double d = static_cast<double>(v[u][e]) - k;
+                const double w = static_cast<double>(g[u][e]) * static_cast<double>(ga[u][e]);
+                s[0] += d; s[1] = fma(d, d, s[1]); s[2] += w; s[3] = fma(w, d, s[3]);
+            }
+        row_fold<G, 4>(s, lds, set);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) { forget(v[u][e]); forget(g[u][e]); forget(ga[u][e]); }
+        const double inv = sh.inv_cols, delta = s[0] * inv, mean = k + delta;
+        const double rstd = row_rstd_fast(row_variance(s[0], s[1], inv), eps);
+        const double w_mean = s[2] * inv, dot = (s[3] - delta * s[2]) * rstd * rstd * inv;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float r[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double d = static_cast<double>(v[u][e]) - mean, gd = static_cast<double>(g[u][e]);
+                const double w = gd * static_cast<double>(ga[u][e]);
+                r[e] = static_cast<float>((w - w_mean - d * dot) * rstd);
+                sg[u][e] = fma(gd, d * rstd, sg[u][e]);
+                sb[u][e] += gd;
+            }
+            if (grad_in) store4(grad_in + at, (u * G + lane) * 4, sh.cols, r);
+        }
+    }
+    if (!partial) return;
+    float* mine = partial + static_cast<uint64_t>(blockIdx.x) * 2 * sh.cols;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int which = 0; which < 2; which++) {
+            double (&t)[4] = which == 0 ? sg[u] : sb[u];
+            if constexpr (groups > 1) {                        // the workgroup's rows side by side, lane by lane
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 4; e++) lds[e * threads + threadIdx.x] = t[e];
+                __syncthreads();
+                if (threadIdx.x < G)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        for (int r = 1; r < groups; r++) t[e] += lds[e * threads + r * G + threadIdx.x];
+            }
+            if (threadIdx.x < G) {
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[e] = static_cast<float>(t[e]);
+                store4(mine + which * sh.cols, (u * G + lane) * 4, sh.cols, f);
+            }
+        }
+}
+
 // ---------------------------------------------------------------- rows in segments (any size)
 
 struct SegPlan {
@@ -244,8 +445,17 @@ __global__ __launch_bounds__(kBlock) void ln_fold_kernel(const float* __restrict
     for (uint32_t c0 = blockIdx.x * kFoldCols; c0 < cols; c0 += gridDim.x * kFoldCols) {
         const uint32_t c = c0 + threadIdx.x % kFoldCols;
         double s = 0.0;
-        if (c < cols)
-            for (uint32_t r = lane; r < ranges; r += kFoldLanes) s += static_cast<double>(partial[(static_cast<uint64_t>(r) * 2 + blockIdx.y) * cols + c]);
+        constexpr uint32_t kAhead = 8;                       // asked for before the first is added
+        for (uint32_t r0 = lane; c < cols && r0 < ranges; r0 += kFoldLanes * kAhead) {
+            float v[kAhead];
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; k++) {
+                const uint32_t r = r0 + k * kFoldLanes;
+                v[k] = r < ranges ? partial[(static_cast<uint64_t>(r) * 2 + blockIdx.y) * cols + c] : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; k++) s += static_cast<double>(v[k]);
+        }
         lds[threadIdx.x] = s;
         __syncthreads();
 #pragma unroll
@@ -293,6 +503,51 @@ SegPlan plan_segments(const Shape2& sh) {
     return pl;
 }
 
+// The widest rows that stay in registers.
+constexpr uint32_t kForwardRowCols = 16384, kBackwardRowCols = 8192;
+
+uint32_t grid_for(const Shape2& sh, uint32_t groups, uint32_t per_unit) {
+    return std::min((sh.rows - 1) / groups + 1, device_units() * per_unit);
+}
+
+template <int G, int U>
+void launch_forward_rows(const Shape2& sh, const float* x, const float* ga, const float* be, float* out, float* mean, float* std, double eps) {
+    constexpr int threads = RowGroup<G>::threads;
+    hipLaunchKernelGGL((ln_forward_rows_kernel<G, U>), dim3(grid_for(sh, RowGroup<G>::groups, 2048 / threads)), dim3(threads), 0, state().stream,
+                       x, ga, be, out, mean, std, sh, eps);
+}
+
+void forward_rows(const Shape2& sh, const float* x, const float* ga, const float* be, float* out, float* mean, float* std, double eps) {
+    const uint32_t c = sh.cols;
+    auto* launch = c <= 16 ? launch_forward_rows<4, 1> : c <= 64 ? launch_forward_rows<16, 1> : c <= 128 ? launch_forward_rows<16, 2>
+                 : c <= 256 ? launch_forward_rows<64, 1> : c <= 512 ? launch_forward_rows<64, 2> : c <= 768 ? launch_forward_rows<64, 3>
+                 : c <= 1024 ? launch_forward_rows<64, 4> : c <= 2048 ? launch_forward_rows<256, 2> : c <= 4096 ? launch_forward_rows<256, 4>
+                 : c <= 8192 ? launch_forward_rows<512, 4> : launch_forward_rows<1024, 4>;
+    launch(sh, x, ga, be, out, mean, std, eps);
+}
+
+struct BackwardRows {
+    void (*kernel)(const float*, const float*, const float*, float*, float*, Shape2, double);
+    uint32_t threads, grid;
+};
+template <int G, int U>
+BackwardRows backward_rows_of(const Shape2& sh, uint32_t per_unit) {
+    return BackwardRows{ln_backward_rows_kernel<G, U>, RowGroup<G>::threads, grid_for(sh, RowGroup<G>::groups, per_unit)};
+}
+BackwardRows backward_rows_kernel(const Shape2& sh) {
+    const uint32_t c = sh.cols;
+    return c <= 16 ? backward_rows_of<4, 1>(sh, 6) : c <= 64 ? backward_rows_of<16, 1>(sh, 6) : c <= 128 ? backward_rows_of<16, 2>(sh, 4)
+         : c <= 256 ? backward_rows_of<64, 1>(sh, 6) : c <= 512 ? backward_rows_of<64, 2>(sh, 4) : c <= 768 ? backward_rows_of<64, 3>(sh, 4)
+         : c <= 1024 ? backward_rows_of<256, 1>(sh, 6) : c <= 2048 ? backward_rows_of<256, 2>(sh, 4) : c <= 4096 ? backward_rows_of<512, 2>(sh, 2)
+         : backward_rows_of<1024, 2>(sh, 1);
+}
+
+void launch_fold(const float* partial, uint32_t cols, uint32_t ranges, float* grad_gamma, float* grad_beta) {
+    LaunchScope scope("ln_fold_kernel", "", static_cast<uint64_t>(ranges) * 2 * cols * sizeof(float));
+    hipLaunchKernelGGL(ln_fold_kernel, dim3(std::min((cols - 1) / kFoldCols + 1, kMaxGrid), 2), dim3(kBlock), 0, state().stream, partial, cols, ranges,
+                       grad_gamma, grad_beta);
+}
+
 uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
 
 }  // namespace
@@ -313,6 +568,12 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
     float* const px = ops[0].ptr; float* const pga = ops[1].ptr; float* const pbe = ops[2].ptr;
     float* const pout = ops[3].ptr; float* const pmean = ops[4].ptr; float* const pstd = ops[5].ptr;
 
+    if (sh.cols <= kForwardRowCols) {
+        LaunchScope scope("ln_forward_rows_kernel", "", n * 8);
+        forward_rows(sh, px, pga, pbe, pout, pmean, pstd, static_cast<double>(epsilon));
+        KTH_LAUNCH_CHECK("layer_norm_forward");
+        return KTH_OK;
+    }
     const SegPlan pl = plan_segments(sh);
     const uint64_t rows_bytes = align256(static_cast<uint64_t>(sh.rows) * sizeof(RowForward));
     const uint64_t blocks = static_cast<uint64_t>(sh.rows) * pl.segments;
@@ -357,6 +618,23 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     float* const px = ops[0].ptr; float* const pga = ops[1].ptr; float* const pgo = ops[2].ptr;
     float* const pgi = ops[3].ptr; float* const pgg = ops[4].ptr; float* const pgb = ops[5].ptr;
 
+    if (sh.cols <= kBackwardRowCols) {
+        const BackwardRows k = backward_rows_kernel(sh);
+        const uint64_t part_bytes = pgg || pgb ? static_cast<uint64_t>(k.grid) * 2 * sh.cols * sizeof(float) : 0;
+        uint64_t part_cap = 0;
+        float* part = part_bytes ? workspace_acquire(part_bytes, &part_cap) : nullptr;
+        if (part_bytes && !part) return fail(KTH_E_MEMORY, "kth_layer_norm_backward: no workspace of %llu bytes", static_cast<unsigned long long>(part_bytes));
+        {
+            LaunchScope scope("ln_backward_rows_kernel", "", n * (pgi ? 12 : 8) + part_bytes);
+            hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pgo, pga, pgi, part, sh, static_cast<double>(epsilon));
+        }
+        if (part) {
+            launch_fold(part, sh.cols, k.grid, pgg, pgb);
+            workspace_release(part, part_cap);
+        }
+        KTH_LAUNCH_CHECK("layer_norm_backward");
+        return KTH_OK;
+    }
     const SegPlan pl = plan_segments(sh);
     ColPlan cp{};
     cp.sh = sh;
@@ -392,11 +670,7 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
         hipLaunchKernelGGL(ln_cols_kernel, dim3(cp.col_blocks * cp.ranges), dim3(kBlock), 0, stream, px, pgo, pga, pgi,
                            rows, partial, cp);
     }
-    if (weights) {
-        LaunchScope scope("ln_fold_kernel", "", cols_bytes);
-        hipLaunchKernelGGL(ln_fold_kernel, dim3(std::min((sh.cols - 1) / kFoldCols + 1, kMaxGrid), 2), dim3(kBlock), 0, stream, partial, sh.cols, cp.ranges,
-                           pgg, pgb);
-    }
+    if (weights) launch_fold(partial, sh.cols, cp.ranges, pgg, pgb);
     workspace_release(reinterpret_cast<float*>(ws), cap);
     KTH_LAUNCH_CHECK("layer_norm_backward");
     return KTH_OK;
