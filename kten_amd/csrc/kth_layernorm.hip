@@ -19,7 +19,6 @@ using namespace kth;
 namespace {
 
 constexpr int kBlock = 256;
-constexpr uint32_t kMaxGrid = 1u << 20;      // (a launch may have fewer than 2^32 threads)
 
 typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));     // 16 bytes at any dword address
 
@@ -73,23 +72,52 @@ __device__ __forceinline__ void block_fold(double (&s)[NS], double* lds) {
 
 // G lanes hold a row, U float4s each (column (u G + lane) 4 + e), so that a pass reads its operands once: a row is summed,
 // its statistics are worked out by every lane, and the results are written from the registers. G = 4, 16 and 64 put
-// several rows into a wave or one, larger G a row into a workgroup; a grid that fills the chip strides over the rows and
-// keeps the weights.
+// several rows into a wave or one, larger G a row into two waves or a workgroup.
 template <int G>
 struct RowGroup {
-    static constexpr int threads = G > kBlock ? G : kBlock;
+    static constexpr int threads = G > 64 ? G : kBlock;      // a row that waves share has the workgroup to itself
     static constexpr int groups = threads / G;                 // rows of a workgroup at a time
     static constexpr int waves = G > 64 ? G / 64 : 0;          // that share a row
 };
+
+// Lane sums of a double without LDS: both halves of the other lane's value by a register move (DPP inside 16 lanes, the
+// row swaps of permlane across them), then an f64 addition. Every step adds the same two values in every lane that takes
+// part, in either order, so all lanes end with the same bits.
+template <int CTRL>
+__device__ __forceinline__ double add_moved(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false);
+    return v + __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double add_row16(double v) {        // rows of 16 lanes: 0 + 1, 2 + 3
+    const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+    const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+    return __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+}
+__device__ __forceinline__ double add_half(double v) {         // the halves of the wave
+    const auto lo = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+    return __hiloint2double(hi[0], lo[0]) + __hiloint2double(hi[1], lo[1]);
+}
+// Over W neighbouring lanes (W = 2, 4, 8, 16: of values that repeat every W lanes of a row of 16 if W < 16; 4: of each quad).
+template <int W>
+__device__ __forceinline__ double lanes_sum(double v) {
+    if constexpr (W == 4) { v = add_moved<0x4e>(v); v = add_moved<0xb1>(v); return v; }      // quad_perm [2,3,0,1], [1,0,3,2]
+    if constexpr (W >= 16) v = add_moved<0x128>(v);                                          // row_ror 8, 4, 2, 1
+    if constexpr (W >= 8) v = add_moved<0x124>(v);
+    if constexpr (W >= 8) v = add_moved<0x122>(v);
+    if constexpr (W >= 2) v = add_moved<0x121>(v);
+    if constexpr (W >= 32) v = add_row16(v);
+    if constexpr (W >= 64) v = add_half(v);
+    return v;
+}
 
 // Sums of NS doubles over the G lanes of a row; every lane gets them, added in the same order. `lds` holds two sets of
 // NS x waves doubles: sets alternate from row to row, so one barrier a row is enough.
 template <int G, int NS>
 __device__ __forceinline__ void row_fold(double (&s)[NS], double* lds, uint32_t& set) {
 #pragma unroll
-    for (int off = (G > 64 ? 64 : G) / 2; off > 0; off >>= 1)
-#pragma unroll
-        for (int i = 0; i < NS; i++) s[i] += __shfl_xor(s[i], off);
+    for (int i = 0; i < NS; i++) s[i] = lanes_sum<(G > 64 ? 64 : G)>(s[i]);
     if constexpr (G > 64) {
         constexpr int waves = RowGroup<G>::waves;
         double* mine = lds + set * NS * waves;
@@ -99,11 +127,7 @@ __device__ __forceinline__ void row_fold(double (&s)[NS], double* lds, uint32_t&
             for (int i = 0; i < NS; i++) mine[i * waves + (threadIdx.x >> 6)] = s[i];
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-            s[i] = mine[i * waves];
-#pragma unroll
-            for (int w = 1; w < waves; w++) s[i] += mine[i * waves + w];
-        }
+        for (int i = 0; i < NS; i++) s[i] = lanes_sum<waves>(mine[i * waves + threadIdx.x % waves]);
     }
 }
 
@@ -114,6 +138,9 @@ __device__ __forceinline__ double row_rstd_fast(double v, double eps) {
     const double y = __builtin_amdgcn_rsq(s);
     return fma(0.5 * y, fma(-s * y, y, 1.0), y);
 }
+
+// Few columns' f64 values at a time, where a lane holds many columns: the compiler would work on all of them at once.
+#define KTH_FEW_AT_A_TIME(e) do { if ((e) % 2 == 1) __builtin_amdgcn_sched_barrier(0); } while (0)
 
 // Four values from column c on; `fill` behind the last column.
 template <bool ONCE>
@@ -158,13 +185,16 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
         const float first = x[at];
         float v[U][4];
 #pragma unroll
-        for (int u = 0; u < U; u++) load4<true>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
+        for (int u = 0; u < U; u++) load4<false>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
         const double k = static_cast<double>(first);
         double s[2] = {};
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) { const double d = static_cast<double>(v[u][e]) - k; s[0] += d; s[1] = fma(d, d, s[1]); }
+            for (int e = 0; e < 4; e++) {
+                const double d = static_cast<double>(v[u][e]) - k;
+                s[0] += d; s[1] = fma(d, d, s[1]);
+            }
         row_fold<G, 2>(s, lds, set);
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -187,10 +217,12 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
 }
 
 // The input gradient of each row, and down the workgroup's rows the weights' gradients, in f64 registers; a workgroup
-// leaves one row [2, cols] of partial sums as floats, each rounded once (2^-24 of itself), which ln_fold_kernel adds in f64.
+// leaves one row [2, cols] of partial sums as floats, each rounded once (2^-24 of itself), which ln_fold_kernel adds in f64;
+// one that is alone (no `partial`) writes the weights' gradients themselves.
 template <int G, int U>
 __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
-                                                                                float* __restrict__ partial, Shape2 sh, double eps) {
+                                                                                float* __restrict__ partial, float* __restrict__ grad_gamma, float* __restrict__ grad_beta,
+                                                                                Shape2 sh, double eps) {
     constexpr int threads = RowGroup<G>::threads, groups = RowGroup<G>::groups;
     __shared__ double lds[G > 64 ? 2 * 4 * RowGroup<G>::waves : threads * 4];
     const uint32_t lane = threadIdx.x % G;
@@ -209,7 +241,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
         float v[U][4], g[U][4];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            load4<true>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
+            load4<false>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
             load4<true>(go + at, (u * G + lane) * 4, sh.cols, 0.0f, g[u]);
         }
         const double k = static_cast<double>(first);
@@ -221,6 +253,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
                 const double d = static_cast<double>(v[u][e]) - k;
                 const double w = static_cast<double>(g[u][e]) * static_cast<double>(ga[u][e]);
                 s[0] += d; s[1] = fma(d, d, s[1]); s[2] += w; s[3] = fma(w, d, s[3]);
+                KTH_FEW_AT_A_TIME(e);
             }
         row_fold<G, 4>(s, lds, set);
 #pragma unroll
@@ -240,11 +273,12 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
                 r[e] = static_cast<float>((w - w_mean - d * dot) * rstd);
                 sg[u][e] = fma(gd, d * rstd, sg[u][e]);
                 sb[u][e] += gd;
+                KTH_FEW_AT_A_TIME(e);
             }
             if (grad_in) store4(grad_in + at, (u * G + lane) * 4, sh.cols, r);
         }
     }
-    if (!partial) return;
+    if (!partial && !grad_gamma && !grad_beta) return;
     float* mine = partial + static_cast<uint64_t>(blockIdx.x) * 2 * sh.cols;
 #pragma unroll
     for (int u = 0; u < U; u++)
@@ -265,17 +299,18 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
                 float f[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) f[e] = static_cast<float>(t[e]);
-                store4(mine + which * sh.cols, (u * G + lane) * 4, sh.cols, f);
+                float* to = partial ? mine + which * sh.cols : which == 0 ? grad_gamma : grad_beta;
+                if (to) store4(to, (u * G + lane) * 4, sh.cols, f);
             }
         }
 }
 
-// ---------------------------------------------------------------- rows in segments (any size)
+// ---------------------------------------------------------------- longer rows, in segments
 
 struct SegPlan {
     Shape2   sh;
     uint32_t segments, seg_len;      // segments per row, columns per segment (a multiple of 4)
-    uint32_t blocks;                 // rows x segments; a grid of at most kMaxGrid workgroups strides over them
+    uint32_t blocks;                 // rows x segments: below 2^19, for the rows are longer than 8192
     FastDiv  seg_div;
 };
 
@@ -285,7 +320,7 @@ __global__ __launch_bounds__(kBlock) void ln_sums_kernel(const float* __restrict
                                                          const float* __restrict__ gamma, double* __restrict__ partial, SegPlan pl) {
     constexpr int NS = BACKWARD ? 4 : 2;
     __shared__ double lds[NS * kBlock / 64];
-    for (uint32_t b = blockIdx.x; b < pl.blocks; b += gridDim.x) {
+    const uint32_t b = blockIdx.x;
     const uint32_t row = divide(b, pl.seg_div);
     const uint32_t seg = b - row * pl.segments;
     const float* xr = x + static_cast<uint64_t>(row) * pl.sh.cols;
@@ -320,8 +355,6 @@ __global__ __launch_bounds__(kBlock) void ln_sums_kernel(const float* __restrict
     if (threadIdx.x == 0)
 #pragma unroll
         for (int i = 0; i < NS; i++) partial[static_cast<uint64_t>(b) * NS + i] = s[i];
-    __syncthreads();
-    }
 }
 
 // One wave per row folds its segments (lane l takes l, l + 64, ...; then the lanes by xor-shuffles).
@@ -330,7 +363,8 @@ __global__ __launch_bounds__(kBlock) void ln_rows_kernel(const float* __restrict
                                                          RowForward* __restrict__ fwd, RowBackward* __restrict__ bwd,
                                                          float* __restrict__ out_mean, float* __restrict__ out_std) {
     constexpr int NS = BACKWARD ? 4 : 2;
-    for (uint32_t row = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6); row < pl.sh.rows; row += gridDim.x * (kBlock / 64)) {
+    const uint32_t row = blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    if (row >= pl.sh.rows) return;
     double s[NS] = {};
     for (uint32_t t = threadIdx.x & 63; t < pl.segments; t += 64)
 #pragma unroll
@@ -339,7 +373,7 @@ __global__ __launch_bounds__(kBlock) void ln_rows_kernel(const float* __restrict
     for (int off = 32; off > 0; off >>= 1)
 #pragma unroll
         for (int i = 0; i < NS; i++) s[i] += __shfl_xor(s[i], off);
-    if ((threadIdx.x & 63) != 0) continue;
+    if ((threadIdx.x & 63) != 0) return;
     const double inv = pl.sh.inv_cols;
     const double delta = s[0] * inv;
     const double mean = static_cast<double>(x[static_cast<uint64_t>(row) * pl.sh.cols]) + delta;
@@ -351,14 +385,12 @@ __global__ __launch_bounds__(kBlock) void ln_rows_kernel(const float* __restrict
         if (out_mean) out_mean[row] = static_cast<float>(mean);
         if (out_std) out_std[row] = static_cast<float>(rstd);
     }
-    }
 }
 
 __global__ __launch_bounds__(kBlock) void ln_apply_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* out,
                                                           const RowForward* __restrict__ fwd, SegPlan pl) {
-    for (uint32_t b = blockIdx.x; b < pl.blocks; b += gridDim.x) {
-    const uint32_t row = divide(b, pl.seg_div);
-    const uint32_t seg = b - row * pl.segments;
+    const uint32_t row = divide(blockIdx.x, pl.seg_div);
+    const uint32_t seg = blockIdx.x - row * pl.segments;
     const uint64_t at = static_cast<uint64_t>(row) * pl.sh.cols;
     const uint32_t first = seg * pl.seg_len;
     const uint32_t last = min(first + pl.seg_len, pl.sh.cols);
@@ -377,7 +409,6 @@ __global__ __launch_bounds__(kBlock) void ln_apply_kernel(const float* x, const 
             for (uint32_t e = c; e < last; e++) out[at + e] = ln_forward(x[at + e], mean, rstd, gamma ? gamma[e] : 1.0f, beta ? beta[e] : 0.0f);
         }
     }
-    }
 }
 
 // ---------------------------------------------------------------- backward by columns
@@ -391,7 +422,8 @@ struct ColPlan {
 // A thread owns four columns of one range of rows: it writes the input gradient of each row and sums the weights'
 // gradients down the range. The partials are floats: each is a f64 sum rounded once (2^-24 of itself), folded in f64.
 __global__ __launch_bounds__(kBlock) void ln_cols_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
-                                                         const RowBackward* __restrict__ rows, float* __restrict__ partial, ColPlan pl) {
+                                                         const RowBackward* __restrict__ rows, float* __restrict__ partial, float* __restrict__ grad_gamma,
+                                                         float* __restrict__ grad_beta, ColPlan pl) {
     const uint32_t range = divide(blockIdx.x, pl.col_div);
     const uint32_t c = ((blockIdx.x - range * pl.col_blocks) * kBlock + threadIdx.x) * 4;
     if (c >= pl.sh.cols) return;
@@ -427,25 +459,32 @@ __global__ __launch_bounds__(kBlock) void ln_cols_kernel(const float* __restrict
                 for (uint32_t e = 0; e < 4; e++) if (e < width) grad_in[at + e] = r[e];
         }
     }
-    if (partial) {
-        float* pg = partial + static_cast<uint64_t>(range) * 2 * pl.sh.cols;
-        for (uint32_t e = 0; e < width; e++) { pg[c + e] = static_cast<float>(sg[e]); pg[pl.sh.cols + c + e] = static_cast<float>(sb[e]); }
+    float* to_gamma = partial ? partial + static_cast<uint64_t>(range) * 2 * pl.sh.cols : grad_gamma;
+    float* to_beta = partial ? to_gamma + pl.sh.cols : grad_beta;
+    for (uint32_t e = 0; e < width; e++) {
+        if (to_gamma) to_gamma[c + e] = static_cast<float>(sg[e]);
+        if (to_beta) to_beta[c + e] = static_cast<float>(sb[e]);
     }
 }
 
-// grad_gamma and grad_beta from `ranges` partial rows of [2, cols]: a workgroup takes 32 columns, eight lanes a column,
-// each with every eighth range; then a tree over the eight. Which of the two sums: blockIdx.y.
-constexpr uint32_t kFoldCols = 32, kFoldLanes = kBlock / kFoldCols;
-__global__ __launch_bounds__(kBlock) void ln_fold_kernel(const float* __restrict__ partial, uint32_t cols, uint32_t ranges,
-                                                         float* __restrict__ grad_gamma, float* __restrict__ grad_beta) {
-    __shared__ double lds[kBlock];
+// grad_gamma and grad_beta from `ranges` partial rows of [2, cols]: a column has kFoldLanes lanes, each with every
+// kFoldLanes-th range, eight of them asked for before the first is added; then a tree over the lanes. Which of the two
+// sums: blockIdx.y. 64 lanes (16 columns a workgroup), or 4 where there are at most 16 ranges (1024 ranges of 768 columns
+// take 7 us with 64 lanes a column, 36 with 8).
+constexpr uint32_t kMaxFoldGrid = 1u << 18;
+constexpr uint32_t kFoldBlock = 1024;
+template <uint32_t kFoldLanes>
+__global__ __launch_bounds__(kFoldBlock) void ln_fold_kernel(const float* __restrict__ partial, uint32_t cols, uint32_t ranges,
+                                                             float* __restrict__ grad_gamma, float* __restrict__ grad_beta) {
+    constexpr uint32_t kFoldCols = kFoldBlock / kFoldLanes;
+    __shared__ double lds[kFoldBlock];
     float* out = blockIdx.y == 0 ? grad_gamma : grad_beta;
     if (!out) return;
     const uint32_t lane = threadIdx.x / kFoldCols;
     for (uint32_t c0 = blockIdx.x * kFoldCols; c0 < cols; c0 += gridDim.x * kFoldCols) {
         const uint32_t c = c0 + threadIdx.x % kFoldCols;
         double s = 0.0;
-        constexpr uint32_t kAhead = 8;                       // asked for before the first is added
+        constexpr uint32_t kAhead = 8;
         for (uint32_t r0 = lane; c < cols && r0 < ranges; r0 += kFoldLanes * kAhead) {
             float v[kAhead];
 #pragma unroll
@@ -503,31 +542,38 @@ SegPlan plan_segments(const Shape2& sh) {
     return pl;
 }
 
-// The widest rows that stay in registers.
+// The widest rows that stay in registers. (With 8 float4s a lane, up to 32768 columns, the forward kernel spills: 82 us for
+// [1000,30000], as much as in segments.)
 constexpr uint32_t kForwardRowCols = 16384, kBackwardRowCols = 8192;
 
 uint32_t grid_for(const Shape2& sh, uint32_t groups, uint32_t per_unit) {
-    return std::min((sh.rows - 1) / groups + 1, device_units() * per_unit);
+    return std::min((sh.rows - 1) / groups + 1, device_units() * per_unit);       // (fewer than 2^32 threads in all)
 }
 
+// A kernel for the rows' width and its grid. Rows of 65 to 2048 columns: a workgroup for each few rows (kOneShot; with
+// workgroups that stride over the rows [65536,1024] takes 98 us instead of 95, [262144,128] 52 instead of 48); shorter and
+// longer ones: so many workgroups a compute unit that stride over the rows and keep the weights ([1000000,33] 82 us instead
+// of 114; [16384,4096] 96 us with 2, 100 with 5, 105 with a workgroup each).
+constexpr uint32_t kOneShot = 1u << 12;
+struct ForwardRows {
+    void (*kernel)(const float*, const float*, const float*, float*, float*, float*, Shape2, double);
+    uint32_t threads, grid;
+};
 template <int G, int U>
-void launch_forward_rows(const Shape2& sh, const float* x, const float* ga, const float* be, float* out, float* mean, float* std, double eps) {
-    constexpr int threads = RowGroup<G>::threads;
-    hipLaunchKernelGGL((ln_forward_rows_kernel<G, U>), dim3(grid_for(sh, RowGroup<G>::groups, 2048 / threads)), dim3(threads), 0, state().stream,
-                       x, ga, be, out, mean, std, sh, eps);
+ForwardRows forward_rows_of(const Shape2& sh, uint32_t per_unit) {
+    return ForwardRows{ln_forward_rows_kernel<G, U>, RowGroup<G>::threads, grid_for(sh, RowGroup<G>::groups, per_unit)};
 }
-
-void forward_rows(const Shape2& sh, const float* x, const float* ga, const float* be, float* out, float* mean, float* std, double eps) {
+ForwardRows forward_rows_kernel(const Shape2& sh) {
     const uint32_t c = sh.cols;
-    auto* launch = c <= 16 ? launch_forward_rows<4, 1> : c <= 64 ? launch_forward_rows<16, 1> : c <= 128 ? launch_forward_rows<16, 2>
-                 : c <= 256 ? launch_forward_rows<64, 1> : c <= 512 ? launch_forward_rows<64, 2> : c <= 768 ? launch_forward_rows<64, 3>
-                 : c <= 1024 ? launch_forward_rows<64, 4> : c <= 2048 ? launch_forward_rows<256, 2> : c <= 4096 ? launch_forward_rows<256, 4>
-                 : c <= 8192 ? launch_forward_rows<512, 4> : launch_forward_rows<1024, 4>;
-    launch(sh, x, ga, be, out, mean, std, eps);
+    return c <= 16 ? forward_rows_of<4, 1>(sh, 8) : c <= 64 ? forward_rows_of<16, 1>(sh, 8) : c <= 128 ? forward_rows_of<16, 2>(sh, kOneShot)
+         : c <= 256 ? forward_rows_of<64, 1>(sh, kOneShot) : c <= 512 ? forward_rows_of<64, 2>(sh, kOneShot)
+         : c <= 768 ? forward_rows_of<64, 3>(sh, kOneShot) : c <= 1024 ? forward_rows_of<64, 4>(sh, kOneShot)
+         : c <= 2048 ? forward_rows_of<128, 4>(sh, kOneShot) : c <= 4096 ? forward_rows_of<256, 4>(sh, 2)
+         : c <= 8192 ? forward_rows_of<512, 4>(sh, 2) : forward_rows_of<1024, 4>(sh, 1);
 }
 
 struct BackwardRows {
-    void (*kernel)(const float*, const float*, const float*, float*, float*, Shape2, double);
+    void (*kernel)(const float*, const float*, const float*, float*, float*, float*, float*, Shape2, double);
     uint32_t threads, grid;
 };
 template <int G, int U>
@@ -536,16 +582,21 @@ BackwardRows backward_rows_of(const Shape2& sh, uint32_t per_unit) {
 }
 BackwardRows backward_rows_kernel(const Shape2& sh) {
     const uint32_t c = sh.cols;
+    // Four float4s a lane are the fastest where there are rows enough for the chip ([65536,1024] 147 us against 217 with
+    // one); with few rows a row is spread over a workgroup.
+    if (c > 512 && c <= 1024 && sh.rows <= 4 * device_units()) return backward_rows_of<256, 1>(sh, 4);
     return c <= 16 ? backward_rows_of<4, 1>(sh, 6) : c <= 64 ? backward_rows_of<16, 1>(sh, 6) : c <= 128 ? backward_rows_of<16, 2>(sh, 4)
-         : c <= 256 ? backward_rows_of<64, 1>(sh, 6) : c <= 512 ? backward_rows_of<64, 2>(sh, 4) : c <= 768 ? backward_rows_of<64, 3>(sh, 4)
-         : c <= 1024 ? backward_rows_of<256, 1>(sh, 6) : c <= 2048 ? backward_rows_of<256, 2>(sh, 4) : c <= 4096 ? backward_rows_of<512, 2>(sh, 2)
+         : c <= 256 ? backward_rows_of<64, 1>(sh, 6) : c <= 512 ? backward_rows_of<64, 2>(sh, 4) : c <= 768 ? backward_rows_of<64, 3>(sh, 3)
+         : c <= 1024 ? backward_rows_of<64, 4>(sh, 2) : c <= 2048 ? backward_rows_of<128, 4>(sh, 4) : c <= 4096 ? backward_rows_of<256, 4>(sh, 2)
          : backward_rows_of<1024, 2>(sh, 1);
 }
 
 void launch_fold(const float* partial, uint32_t cols, uint32_t ranges, float* grad_gamma, float* grad_beta) {
     LaunchScope scope("ln_fold_kernel", "", static_cast<uint64_t>(ranges) * 2 * cols * sizeof(float));
-    hipLaunchKernelGGL(ln_fold_kernel, dim3(std::min((cols - 1) / kFoldCols + 1, kMaxGrid), 2), dim3(kBlock), 0, state().stream, partial, cols, ranges,
-                       grad_gamma, grad_beta);
+    const uint32_t lanes = ranges <= 16 ? 4 : 64, per_block = kFoldBlock / lanes;
+    const dim3 grid(std::min((cols - 1) / per_block + 1, kMaxFoldGrid), 2);
+    if (lanes == 4) hipLaunchKernelGGL((ln_fold_kernel<4>), grid, dim3(kFoldBlock), 0, state().stream, partial, cols, ranges, grad_gamma, grad_beta);
+    else            hipLaunchKernelGGL((ln_fold_kernel<64>), grid, dim3(kFoldBlock), 0, state().stream, partial, cols, ranges, grad_gamma, grad_beta);
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
@@ -570,7 +621,8 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
 
     if (sh.cols <= kForwardRowCols) {
         LaunchScope scope("ln_forward_rows_kernel", "", n * 8);
-        forward_rows(sh, px, pga, pbe, pout, pmean, pstd, static_cast<double>(epsilon));
+        const ForwardRows k = forward_rows_kernel(sh);
+        hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pga, pbe, pout, pmean, pstd, sh, static_cast<double>(epsilon));
         KTH_LAUNCH_CHECK("layer_norm_forward");
         return KTH_OK;
     }
@@ -586,16 +638,16 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
     hipStream_t stream = state().stream;
     {
         LaunchScope scope("ln_sums_kernel", "forward", n * 4);
-        hipLaunchKernelGGL((ln_sums_kernel<false>), dim3(std::min(pl.blocks, kMaxGrid)), dim3(kBlock), 0, stream, px, nullptr, nullptr, partial, pl);
+        hipLaunchKernelGGL((ln_sums_kernel<false>), dim3(pl.blocks), dim3(kBlock), 0, stream, px, nullptr, nullptr, partial, pl);
     }
     {
         LaunchScope scope("ln_rows_kernel", "forward", blocks * 16);
-        hipLaunchKernelGGL((ln_rows_kernel<false>), dim3(std::min((sh.rows - 1) / 4 + 1, kMaxGrid)), dim3(kBlock), 0, stream, px, partial, pl, static_cast<double>(epsilon),
+        hipLaunchKernelGGL((ln_rows_kernel<false>), dim3((sh.rows - 1) / 4 + 1), dim3(kBlock), 0, stream, px, partial, pl, static_cast<double>(epsilon),
                            rows, nullptr, pmean, pstd);
     }
     {
         LaunchScope scope("ln_apply_kernel", "", n * 8);
-        hipLaunchKernelGGL(ln_apply_kernel, dim3(std::min(pl.blocks, kMaxGrid)), dim3(kBlock), 0, stream, px, pga,
+        hipLaunchKernelGGL(ln_apply_kernel, dim3(pl.blocks), dim3(kBlock), 0, stream, px, pga,
                            pbe, pout, rows, pl);
     }
     workspace_release(reinterpret_cast<float*>(ws), cap);
@@ -620,13 +672,13 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
 
     if (sh.cols <= kBackwardRowCols) {
         const BackwardRows k = backward_rows_kernel(sh);
-        const uint64_t part_bytes = pgg || pgb ? static_cast<uint64_t>(k.grid) * 2 * sh.cols * sizeof(float) : 0;
+        const uint64_t part_bytes = (pgg || pgb) && k.grid > 1 ? static_cast<uint64_t>(k.grid) * 2 * sh.cols * sizeof(float) : 0;
         uint64_t part_cap = 0;
         float* part = part_bytes ? workspace_acquire(part_bytes, &part_cap) : nullptr;
         if (part_bytes && !part) return fail(KTH_E_MEMORY, "kth_layer_norm_backward: no workspace of %llu bytes", static_cast<unsigned long long>(part_bytes));
         {
             LaunchScope scope("ln_backward_rows_kernel", "", n * (pgi ? 12 : 8) + part_bytes);
-            hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pgo, pga, pgi, part, sh, static_cast<double>(epsilon));
+            hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pgo, pga, pgi, part, part ? nullptr : pgg, part ? nullptr : pgb, sh, static_cast<double>(epsilon));
         }
         if (part) {
             launch_fold(part, sh.cols, k.grid, pgg, pgb);
@@ -643,7 +695,7 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     cp.rows_per_range = (sh.rows + cp.ranges - 1) / cp.ranges;
     cp.ranges = (sh.rows + cp.rows_per_range - 1) / cp.rows_per_range;
     cp.col_div = make_div(cp.col_blocks);
-    const bool weights = pgg || pgb;
+    const bool weights = (pgg || pgb) && cp.ranges > 1;
     const uint64_t blocks = static_cast<uint64_t>(sh.rows) * pl.segments;
     const uint64_t rows_bytes = align256(static_cast<uint64_t>(sh.rows) * sizeof(RowBackward));
     const uint64_t sums_bytes = align256(blocks * 4 * sizeof(double));
@@ -658,17 +710,17 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     hipStream_t stream = state().stream;
     {
         LaunchScope scope("ln_sums_kernel", "backward", n * 8);
-        hipLaunchKernelGGL((ln_sums_kernel<true>), dim3(std::min(pl.blocks, kMaxGrid)), dim3(kBlock), 0, stream, px, pgo, pga, sums, pl);
+        hipLaunchKernelGGL((ln_sums_kernel<true>), dim3(pl.blocks), dim3(kBlock), 0, stream, px, pgo, pga, sums, pl);
     }
     {
         LaunchScope scope("ln_rows_kernel", "backward", blocks * 32);
-        hipLaunchKernelGGL((ln_rows_kernel<true>), dim3(std::min((sh.rows - 1) / 4 + 1, kMaxGrid)), dim3(kBlock), 0, stream, px, sums, pl, static_cast<double>(epsilon),
+        hipLaunchKernelGGL((ln_rows_kernel<true>), dim3((sh.rows - 1) / 4 + 1), dim3(kBlock), 0, stream, px, sums, pl, static_cast<double>(epsilon),
                            nullptr, rows, nullptr, nullptr);
     }
     {
         LaunchScope scope("ln_cols_kernel", "", n * (pgi ? 12 : 8) + cols_bytes);
         hipLaunchKernelGGL(ln_cols_kernel, dim3(cp.col_blocks * cp.ranges), dim3(kBlock), 0, stream, px, pgo, pga, pgi,
-                           rows, partial, cp);
+                           rows, partial, weights ? nullptr : pgg, weights ? nullptr : pgb, cp);
     }
     if (weights) launch_fold(partial, sh.cols, cp.ranges, pgg, pgb);
     workspace_release(reinterpret_cast<float*>(ws), cap);
