@@ -372,6 +372,254 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
     if (grad_initial && w.valid && q0 < pl.steps && q0 + L >= pl.steps) grad_initial[w.first_state] = static_cast<float>(K);
 }
 
+// ---------------------------------------------------------------- few channels side by side
+
+// With fewer than 32 channels side by side (inner) a wave's lanes would each walk memory of their own. Here a workgroup
+// takes a stretch of up to 4096 floats as memory has them, through LDS, and a thread kSub steps of one channel: thread
+// (row, j, channel), j counting the kSub-step pieces of a row. Rows that fit are taken several at a time; longer ones are
+// cut into tiles that hand a state on as above. A piece's place in LDS is padded by one float, so that the threads of a
+// wave, a piece apart, do not meet in a bank.
+constexpr uint32_t kNarrowThreads = 256, kSub = 16, kNarrowInner = 32;
+constexpr uint32_t kNarrowFloats = kNarrowThreads * (kSub + 1);
+
+struct NarrowPlan {
+    uint32_t outer, steps, inner;
+    uint32_t rows;                   // outer indices of a workgroup (1 if tiles > 1)
+    uint32_t pieces;                 // of kSub steps, of a row in a workgroup
+    uint32_t tile_steps, tiles;
+    uint32_t channels;               // outer x inner
+    uint32_t tag, ticket_base;
+    uint32_t* tickets;
+    uint64_t* pairs;                 // [tiles][channels][2]
+    uint64_t* states;                // [tiles / kSuper][channels]
+    FastDiv  inner_div, row_div, outer_div, piece_div;     // row_div divides by the floats of a row of this workgroup
+};
+
+struct NarrowPlace {
+    uint32_t tile, o0, rows;         // first outer index and how many
+    uint32_t q0, count;              // first step (counted in the scan's direction) and how many
+    uint32_t r, j, c;                // this thread's
+    bool     works;
+    uint32_t channel;                // of all, this thread's
+};
+
+__device__ __forceinline__ bool place_narrow(const NarrowPlan& pl, uint32_t* lds_ticket, NarrowPlace& w) {
+    uint32_t ticket = blockIdx.x;
+    if (pl.tiles > 1) {
+        if (threadIdx.x == 0) *lds_ticket = atomicAdd(pl.tickets, 1u) - pl.ticket_base;
+        __syncthreads();
+        ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
+        if (ticket >= pl.tiles * pl.outer) return false;
+        w.tile = divide(ticket, pl.outer_div);
+        w.o0 = ticket - w.tile * pl.outer;
+        w.rows = 1;
+    } else {
+        w.tile = 0;
+        w.o0 = ticket * pl.rows;
+        w.rows = min(pl.rows, pl.outer - w.o0);
+    }
+    w.q0 = w.tile * pl.tile_steps;
+    w.count = min(pl.tile_steps, pl.steps - w.q0);
+    const uint32_t piece = divide(threadIdx.x, pl.inner_div);          // row and j together
+    w.c = threadIdx.x - piece * pl.inner;
+    w.r = divide(piece, pl.piece_div);
+    w.j = piece - w.r * pl.pieces;
+    w.works = w.r < w.rows;
+    w.channel = (w.o0 + w.r) * pl.inner + w.c;
+    return true;
+}
+
+// Where the float e of the workgroup's stretch lies in memory and in LDS. REVERSE: steps are counted from the last one.
+template <bool REVERSE>
+__device__ __forceinline__ uint64_t narrow_index(const NarrowPlan& pl, const NarrowPlace& w, uint32_t e, uint32_t& place) {
+    const uint32_t r = w.rows > 1 ? divide(e, pl.row_div) : 0;
+    const uint32_t in_row = e - r * (w.count * pl.inner);
+    const uint32_t t = divide(in_row, pl.inner_div);
+    const uint32_t c = in_row - t * pl.inner;
+    const uint32_t s = REVERSE ? w.count - 1 - t : t;                  // in the scan's order
+    place = (r * pl.pieces + s / kSub) * (kSub * pl.inner + 1) + (s % kSub) * pl.inner + c;
+    const uint32_t first = REVERSE ? pl.steps - w.q0 - w.count : w.q0;
+    return (static_cast<uint64_t>(w.o0 + r) * pl.steps + first + t) * pl.inner + c;
+}
+
+// The state before this thread's piece from the piece's pair (A, H); `initial` is its channel's, read by the first piece of
+// the first tile. pair: kNarrowThreads pairs of LDS; handed: kSuper x inner more, and inner states.
+__device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, const NarrowPlace& w, double A, double H, double initial,
+                                                      Pair* pair, Pair* handed, double* carried) {
+    Pair mine = w.works ? Pair{A, H} : Pair{1.0, 0.0};
+    if (w.works && w.tile == 0 && w.j == 0) mine = Pair{0.0, advance(A, H, initial)};   // nobody else reads `initial`
+    for (uint32_t d = 1; d < pl.pieces; d <<= 1) {                     // pieces up to and with this one
+        pair[threadIdx.x] = mine;
+        __syncthreads();
+        if (w.works && w.j >= d) {
+            const Pair p = pair[threadIdx.x - d * pl.inner];
+            mine = Pair{mine.A * p.A, advance(mine.A, mine.H, p.H)};
+        }
+        __syncthreads();
+    }
+    pair[threadIdx.x] = mine;
+    __syncthreads();
+    double state = 0.0;
+    if (pl.tiles > 1) {
+        const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
+        const Pair* total = pair + (pl.pieces - 1) * pl.inner;        // (a tile that is cut short is the last: nobody reads its total)
+        if (threadIdx.x < pl.inner && w.tile + 1 < pl.tiles && many + 1 < kSuper) {
+            uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.channels + w.o0 * pl.inner + threadIdx.x) * 2;
+            publish(word, total[threadIdx.x].A, pl.tag);
+            publish(word + 1, total[threadIdx.x].H, pl.tag);
+        }
+        if (w.tile > 0) {
+            for (uint32_t i = threadIdx.x; i < many * pl.inner; i += kNarrowThreads) {
+                const uint32_t t = divide(i, pl.inner_div);
+                const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + t) * pl.channels + w.o0 * pl.inner + (i - t * pl.inner)) * 2;
+                const double a = await(word, pl.tag), h = await(word + 1, pl.tag);
+                handed[i] = Pair{a, h};
+            }
+            __syncthreads();
+            if (threadIdx.x < pl.inner) {
+                const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
+                double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.tag);
+                for (uint32_t t = 0; t < many; t++) { const Pair p = handed[t * pl.inner + threadIdx.x]; s = advance(p.A, p.H, s); }
+                carried[threadIdx.x] = s;
+                if (many + 1 == kSuper && w.tile + 1 < pl.tiles)
+                    publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance(total[threadIdx.x].A, total[threadIdx.x].H, s), pl.tag);
+            }
+            __syncthreads();
+            state = carried[w.c];
+        }
+    }
+    if (w.tile == 0 && w.j == 0) return initial;
+    if (w.j == 0) return state;
+    const Pair p = pair[threadIdx.x - pl.inner];
+    return advance(p.A, p.H, state);
+}
+
+// LDS of both kernels: two stretches of floats, the pairs, what earlier tiles handed on.
+struct NarrowShared {
+    float  a[kNarrowFloats], b[kNarrowFloats];
+    Pair   pair[kNarrowThreads];
+    Pair   handed[kSuper * kNarrowInner];
+    double carried[kNarrowInner];
+    uint32_t ticket;
+};
+
+template <bool SIGMOID>
+__global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kernel(const float* __restrict__ gate, const float* __restrict__ in, const float* initial,
+                                                                                   float* __restrict__ out, float* final_state, NarrowPlan pl) {
+    __shared__ NarrowShared sh;
+    NarrowPlace w;
+    if (!place_narrow(pl, &sh.ticket, w)) return;
+    const uint32_t floats = w.rows * w.count * pl.inner;
+#pragma unroll 8
+    for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
+        uint32_t place;
+        const uint64_t at = narrow_index<false>(pl, w, e, place);
+        sh.a[place] = gate[at];
+        sh.b[place] = in[at];
+    }
+    const double start = w.works && w.tile == 0 && w.j == 0 && initial ? static_cast<double>(initial[w.channel]) : 0.0;
+    __syncthreads();
+    const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
+    const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
+    double A = 1.0, H = 0.0;
+    for (uint32_t k = 0; k < count; k++) {
+        const uint32_t i = base + k * pl.inner;
+        const float v = pack_gate<SIGMOID>(sh.a[i]);
+        const float u = SIGMOID ? sigmoid_b(v) * sh.b[i] : sh.b[i];
+        if (SIGMOID) { sh.a[i] = v; sh.b[i] = u; }
+        const double a = gate_a<SIGMOID>(v);
+        H = fma(a, H, static_cast<double>(u));
+        A *= a;
+    }
+    double h = narrow_state_before(pl, w, A, H, start, sh.pair, sh.handed, sh.carried);
+    for (uint32_t k = 0; k < count; k++) {
+        const uint32_t i = base + k * pl.inner;
+        h = fma(gate_a<SIGMOID>(sh.a[i]), h, static_cast<double>(sh.b[i]));
+        sh.b[i] = static_cast<float>(h);
+    }
+    if (final_state && count > 0 && w.q0 + w.j * kSub + count == pl.steps) final_state[w.channel] = static_cast<float>(h);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
+        uint32_t place;
+        const uint64_t at = narrow_index<false>(pl, w, e, place);
+        out[at] = sh.b[place];
+    }
+}
+
+template <bool SIGMOID>
+__global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_kernel(const float* __restrict__ gate, const float* __restrict__ in,
+                                                                                    const float* __restrict__ initial, const float* __restrict__ out,
+                                                                                    const float* __restrict__ grad_out, const float* __restrict__ grad_final,
+                                                                                    float* __restrict__ grad_gate, float* __restrict__ grad_in,
+                                                                                    float* __restrict__ grad_initial, NarrowPlan pl) {
+    __shared__ NarrowShared sh;
+    NarrowPlace w;
+    if (!place_narrow(pl, &sh.ticket, w)) return;
+    const uint32_t floats = w.rows * w.count * pl.inner;
+#pragma unroll 8
+    for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
+        uint32_t place;
+        const uint64_t at = narrow_index<true>(pl, w, e, place);
+        sh.a[place] = gate[at];
+        sh.b[place] = grad_out[at];
+    }
+    const double start = w.works && w.tile == 0 && w.j == 0 && grad_final ? static_cast<double>(grad_final[w.channel]) : 0.0;
+    __syncthreads();
+    const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
+    const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
+    double A = 1.0, H = 0.0;
+    float v[kSub], g[kSub];
+#pragma unroll
+    for (uint32_t k = 0; k < kSub; k++) {
+        if (k < count) {
+            const uint32_t i = base + k * pl.inner;
+            v[k] = pack_gate<SIGMOID>(sh.a[i]);
+            g[k] = sh.b[i];
+            const double a = gate_a<SIGMOID>(v[k]);
+            H = a * (static_cast<double>(g[k]) + H);
+            A *= a;
+        }
+    }
+    double K = narrow_state_before(pl, w, A, H, start, sh.pair, sh.handed, sh.carried);
+    __syncthreads();                                                   // gate and grad_out are in registers: their LDS is free
+    if (grad_gate) {                                                   // (without it out and in need not be given)
+#pragma unroll 8
+        for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
+            uint32_t place;
+            const uint64_t at = narrow_index<true>(pl, w, e, place);
+            // the state before the step; before the first step of a row it is `initial`
+            const uint32_t r = w.rows > 1 ? divide(e, pl.row_div) : 0;
+            const uint32_t t = e - r * (w.count * pl.inner);
+            const bool first = t < pl.inner && w.q0 + w.count == pl.steps;
+            sh.a[place] = !first ? out[at - pl.inner] : initial ? initial[(w.o0 + r) * pl.inner + t] : 0.0f;
+            if (SIGMOID) sh.b[place] = in[at];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kSub; k++) {
+        if (k < count) {
+            const uint32_t i = base + k * pl.inner;
+            const double a = gate_a<SIGMOID>(v[k]), b = SIGMOID ? static_cast<double>(sigmoid_b(v[k])) : 1.0;
+            const double d = static_cast<double>(g[k]) + K;
+            if (grad_gate) {
+                const double before = static_cast<double>(sh.a[i]);
+                sh.a[i] = static_cast<float>(SIGMOID ? d * (before - static_cast<double>(sh.b[i])) * (a * b) : d * before);
+            }
+            sh.b[i] = static_cast<float>(d * b);
+            K = a * d;
+        }
+    }
+    if (grad_initial && count > 0 && w.q0 + w.j * kSub + count == pl.steps) grad_initial[w.channel] = static_cast<float>(K);
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
+        uint32_t place;
+        const uint64_t at = narrow_index<true>(pl, w, e, place);
+        if (grad_gate) grad_gate[at] = sh.a[place];
+        if (grad_in) grad_in[at] = sh.b[place];
+    }
+}
+
 // ---------------------------------------------------------------- host side
 
 // Up to here a thread walks all steps of its channel.
@@ -379,6 +627,36 @@ constexpr uint32_t kShortForward = 32, kShortBackward = 4;
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
 // one stream, and each has a tag and a range of tickets of its own.
+int take_words(const char* what, uint64_t words, uint32_t tickets, uint32_t* tag, uint32_t* ticket_base, uint32_t** counter, uint64_t** first) {
+    constexpr uint64_t kHead = 64;                           // the ticket counter, on cache lines of its own
+    State& s = state();
+    words += kHead;
+    if (words > s.scan_words || s.scan_tag == kTags) {
+        if (words > s.scan_words) {
+            KTH_HIP(hipStreamSynchronize(s.stream));
+            if (s.scan) KTH_HIP(hipFree(s.scan));
+            s.scan = nullptr; s.scan_words = 0;
+            void* p = nullptr;
+            if (hipMalloc(&p, words * 8) != hipSuccess) {
+                (void)hipGetLastError();
+                return fail(KTH_E_MEMORY, "%s: no workspace of %llu bytes", what, static_cast<unsigned long long>(words * 8));
+            }
+            s.scan = static_cast<uint64_t*>(p);
+            s.scan_words = words;
+        }
+        for (uint64_t at = 0; at < s.scan_words; at += 1ull << 29)
+            launch_fill(reinterpret_cast<float*>(s.scan + at), 2 * std::min<uint64_t>(s.scan_words - at, 1ull << 29), 0.0f);
+        s.scan_tag = 0; s.scan_tickets = 0;
+    }
+    s.scan_tag += 1;
+    *tag = s.scan_tag;
+    *ticket_base = s.scan_tickets;
+    s.scan_tickets += tickets;                               // (wraps, as the counter does)
+    *counter = reinterpret_cast<uint32_t*>(s.scan);
+    *first = s.scan + kHead;
+    return KTH_OK;
+}
+
 int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     TilePlan pl{};
     pl.steps = sh.steps; pl.inner = sh.inner;
@@ -390,39 +668,41 @@ int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     pl.group_div = make_div(pl.groups);
     pl.col_div = make_div(pl.col_blocks);
     if (pl.tiles > 1) {
-        State& s = state();
         const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.padded * 2;
-        const uint64_t words = 64 + pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded;
-        if (words > s.scan_words || s.scan_tag == kTags) {
-            if (words > s.scan_words) {
-                KTH_HIP(hipStreamSynchronize(s.stream));
-                if (s.scan) KTH_HIP(hipFree(s.scan));
-                s.scan = nullptr; s.scan_words = 0;
-                void* p = nullptr;
-                if (hipMalloc(&p, words * 8) != hipSuccess) {
-                    (void)hipGetLastError();
-                    return fail(KTH_E_MEMORY, "%s: no workspace of %llu bytes", what, static_cast<unsigned long long>(words * 8));
-                }
-                s.scan = static_cast<uint64_t*>(p);
-                s.scan_words = words;
-            }
-            for (uint64_t at = 0; at < s.scan_words; at += 1ull << 29)
-                launch_fill(reinterpret_cast<float*>(s.scan + at), 2 * std::min<uint64_t>(s.scan_words - at, 1ull << 29), 0.0f);
-            s.scan_tag = 0; s.scan_tickets = 0;
-        }
-        s.scan_tag += 1;
-        pl.tag = s.scan_tag;
-        pl.ticket_base = s.scan_tickets;
-        s.scan_tickets += pl.tiles * pl.groups;              // (wraps, as the counter does)
-        pl.tickets = reinterpret_cast<uint32_t*>(s.scan);
-        pl.pairs = s.scan + 64;
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded, pl.tiles * pl.groups, &pl.tag, &pl.ticket_base,
+                                &pl.tickets, &pl.pairs)) return rc;
         pl.states = pl.pairs + pairs;
     }
     *out = pl;
     return KTH_OK;
 }
 
-// A launch that failed drew no tickets: the next one starts from cleared words.
+int plan_narrow(const char* what, const ScanShape& sh, NarrowPlan* out, uint32_t* grid) {
+    NarrowPlan pl{};
+    pl.outer = sh.outer; pl.steps = sh.steps; pl.inner = sh.inner; pl.channels = sh.channels;
+    const uint32_t most = kNarrowThreads / sh.inner;         // pieces of a workgroup
+    const uint32_t pieces = (sh.steps - 1) / kSub + 1;
+    pl.pieces = std::min(pieces, most);
+    pl.rows = std::min(sh.outer, most / pl.pieces);
+    pl.tile_steps = pieces <= most ? sh.steps : most * kSub;
+    pl.tiles = (sh.steps - 1) / pl.tile_steps + 1;
+    if (pl.tiles > 1) pl.rows = 1;
+    pl.inner_div = make_div(sh.inner);
+    pl.row_div = make_div(sh.steps * sh.inner);              // (used where whole rows are taken)
+    pl.outer_div = make_div(sh.outer);
+    pl.piece_div = make_div(pl.pieces);
+    *grid = pl.tiles > 1 ? pl.tiles * sh.outer : (sh.outer - 1) / pl.rows + 1;
+    if (pl.tiles > 1) {
+        const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.channels * 2;
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.channels, *grid, &pl.tag, &pl.ticket_base, &pl.tickets,
+                                &pl.pairs)) return rc;
+        pl.states = pl.pairs + pairs;
+    }
+    *out = pl;
+    return KTH_OK;
+}
+
+// (as KTH_LAUNCH_CHECK) A launch that failed drew no tickets: the next one starts from cleared words.
 int tiles_launched(const char* what) {
     const hipError_t e = hipGetLastError();
     if (e == hipSuccess) return KTH_OK;
@@ -470,7 +750,15 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
                       {"out", out, n, true}, {"final_state", final_state, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 5, {{4, 2}})) return rc;          // the state may be updated in place
     const bool sigmoid = mode == KTH_GATE_SIGMOID;
-    if (sh.steps > kShortForward && sh.inner >= 32) {
+    if (sh.steps > 1 && sh.inner < kNarrowInner) {
+        NarrowPlan pl; uint32_t grid;
+        if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
+        LaunchScope scope("recurrence_forward_narrow_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
+        auto* kernel = sigmoid ? recurrence_forward_narrow_kernel<true> : recurrence_forward_narrow_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
+        return tiles_launched("gated_recurrence_forward");
+    }
+    if (sh.steps > kShortForward) {
         constexpr int L = 32;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
@@ -510,7 +798,16 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                       {"grad_gate", grad_gate, n, true}, {"grad_in", grad_in, n, true},
                       {"grad_initial", grad_initial, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 9, {})) return rc;
-    if (sh.steps > kShortBackward && sh.inner >= 32) {
+    if (sh.steps > 1 && sh.inner < kNarrowInner) {
+        NarrowPlan pl; uint32_t grid;
+        if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
+        LaunchScope scope("recurrence_backward_narrow_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
+        auto* kernel = sigmoid ? recurrence_backward_narrow_kernel<true> : recurrence_backward_narrow_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
+                           ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
+        return tiles_launched("gated_recurrence_backward");
+    }
+    if (sh.steps > kShortBackward) {
         constexpr int L = 16;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
