@@ -100,19 +100,35 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
     const uint64_t first = static_cast<uint64_t>(o) * sh.steps * sh.inner + (ch - o * sh.inner);
     const float h0 = initial ? initial[ch] : 0.0f;
     double carry = grad_final ? static_cast<double>(grad_final[ch]) : 0.0;      // a_{t+1} d_{t+1}
-    for (uint32_t left = sh.steps; left > 0; left--) {
-        const uint32_t t = left - 1;
-        const uint64_t at = first + static_cast<uint64_t>(t) * sh.inner;
-        const float v = pack_gate<SIGMOID>(gate[at]);
-        const double a = gate_a<SIGMOID>(v), b = SIGMOID ? static_cast<double>(sigmoid_b(v)) : 1.0;
-        const double d = static_cast<double>(grad_out[at]) + carry;
-        if (grad_gate) {                                 // (without it out and in need not be given)
-            const float before = t > 0 ? out[at - sh.inner] : h0;
-            grad_gate[at] = static_cast<float>(SIGMOID ? d * (static_cast<double>(before) - static_cast<double>(in[at])) * (a * b)
-                                                       : d * static_cast<double>(before));
+    for (uint32_t left = sh.steps; left > 0; left -= min(left, static_cast<uint32_t>(kAhead))) {
+        // steps left - 1, left - 2, ...; what only the gate's gradient needs (without it out and in need not be given) too
+        float v[kAhead], g[kAhead], before[kAhead], x[kAhead];
+        const uint64_t top = first + static_cast<uint64_t>(left - 1) * sh.inner;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const uint64_t at = top - static_cast<uint64_t>(k) * sh.inner;
+            if (static_cast<uint32_t>(k) < left) {
+                v[k] = gate[at]; g[k] = grad_out[at];
+                if (grad_gate) {
+                    before[k] = static_cast<uint32_t>(k) + 1 < left ? out[at - sh.inner] : h0;
+                    if (SIGMOID) x[k] = in[at];
+                }
+            }
         }
-        if (grad_in) grad_in[at] = static_cast<float>(d * b);
-        carry = a * d;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const uint64_t at = top - static_cast<uint64_t>(k) * sh.inner;
+            if (static_cast<uint32_t>(k) < left) {
+                const float p = pack_gate<SIGMOID>(v[k]);
+                const double a = gate_a<SIGMOID>(p), b = SIGMOID ? static_cast<double>(sigmoid_b(p)) : 1.0;
+                const double d = static_cast<double>(g[k]) + carry;
+                if (grad_gate)
+                    grad_gate[at] = static_cast<float>(SIGMOID ? d * (static_cast<double>(before[k]) - static_cast<double>(x[k])) * (a * b)
+                                                               : d * static_cast<double>(before[k]));
+                if (grad_in) grad_in[at] = static_cast<float>(d * b);
+                carry = a * d;
+            }
+        }
     }
     if (grad_initial) grad_initial[ch] = static_cast<float>(carry);
 }
@@ -374,12 +390,12 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
 
 // ---------------------------------------------------------------- few channels side by side
 
-// With fewer than 32 channels side by side (inner) a wave's lanes would each walk memory of their own. Here a workgroup
+// With few channels side by side (inner) a wave's lanes would each walk memory of their own. Here a workgroup
 // takes a stretch of up to 4096 floats as memory has them, through LDS, and a thread kSub steps of one channel: thread
 // (row, j, channel), j counting the kSub-step pieces of a row. Rows that fit are taken several at a time; longer ones are
 // cut into tiles that hand a state on as above. A piece's place in LDS is padded by one float, so that the threads of a
 // wave, a piece apart, do not meet in a bank.
-constexpr uint32_t kNarrowThreads = 256, kSub = 16, kNarrowInner = 32;
+constexpr uint32_t kNarrowThreads = 256, kSub = 16, kNarrowInner = 32;     // (inner is below kNarrowInner)
 constexpr uint32_t kNarrowFloats = kNarrowThreads * (kSub + 1);
 
 struct NarrowPlan {
@@ -622,8 +638,21 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
 
 // ---------------------------------------------------------------- host side
 
-// Up to here a thread walks all steps of its channel.
-constexpr uint32_t kShortForward = 32, kShortBackward = 4;
+// Which kernel takes a call. Times in us, sigmoid gates, walk / tiles / narrow:
+//   few steps: [64,8,1024] 3.9 / 5.9 forward and 5.9 / 6.3 backward, [64,16,1024] 4.7 / 6.6 and 11.4 / 9.2,
+//     [64,32,1024] 8.5 / 9.0 and 19.8 / 12.1; [1000,8,3] 4.1 / 5.6 / 7.0 and 6.0 / 5.5 / 12.5;
+//   many channels, few side by side: [20000,32,8] 13 / 53 / 30 and 44 / 88 / 74, [100000,20,24] forward 126 / - / 311;
+//   hardly any side by side: [100000,64,1] 85 / 421 / 38 and 354 / 735 / 101, [1,66000,2] 4419 / - / 13;
+//   otherwise [1000,100,20] 18 / 14 / 21 and 61 / 21 / 34, [100,100,5] 18 / 6 / 10 and 44 / 7.5 / 15.
+enum class Path { walk, tiles, narrow };
+Path path_of(const ScanShape& sh, bool forward) {
+    const uint32_t few = forward && sh.inner >= 8 ? 32 : 8;
+    if (sh.steps <= few) return Path::walk;
+    if (sh.inner >= kNarrowInner) return Path::tiles;
+    if (sh.inner >= 8) return sh.channels >= (1u << 17) ? Path::walk : Path::tiles;
+    if (sh.inner >= 4 && static_cast<uint64_t>(sh.channels) * sh.steps < (1u << 20)) return Path::tiles;
+    return Path::narrow;
+}
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
 // one stream, and each has a tag and a range of tickets of its own.
@@ -750,7 +779,8 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
                       {"out", out, n, true}, {"final_state", final_state, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 5, {{4, 2}})) return rc;          // the state may be updated in place
     const bool sigmoid = mode == KTH_GATE_SIGMOID;
-    if (sh.steps > 1 && sh.inner < kNarrowInner) {
+    const Path path = path_of(sh, true);
+    if (path == Path::narrow) {
         NarrowPlan pl; uint32_t grid;
         if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
         LaunchScope scope("recurrence_forward_narrow_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
@@ -758,7 +788,7 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
         return tiles_launched("gated_recurrence_forward");
     }
-    if (sh.steps > kShortForward) {
+    if (path == Path::tiles) {
         constexpr int L = 32;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
@@ -798,7 +828,8 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                       {"grad_gate", grad_gate, n, true}, {"grad_in", grad_in, n, true},
                       {"grad_initial", grad_initial, sh.channels, true}};
     if (int rc = resolve_operands(what, ops, 9, {})) return rc;
-    if (sh.steps > 1 && sh.inner < kNarrowInner) {
+    const Path path = path_of(sh, false);
+    if (path == Path::narrow) {
         NarrowPlan pl; uint32_t grid;
         if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
         LaunchScope scope("recurrence_backward_narrow_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
@@ -807,7 +838,7 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                            ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
         return tiles_launched("gated_recurrence_backward");
     }
-    if (sh.steps > kShortBackward) {
+    if (path == Path::tiles) {
         constexpr int L = 16;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;

@@ -205,6 +205,60 @@ def test_the_same_call_gives_the_same_bits(gc):
                 assert_bits_equal(a, b, "the same call again")
 
 
+@pytest.mark.parametrize("sigmoid", [True, False], ids=["sigmoid", "given"])
+@pytest.mark.parametrize("shape", [(20000, 33, 8), (9000, 60, 15), (70000, 11, 4), (3, 100000, 7), (40, 5000, 4), (257, 300, 31), (1, 200, 31), (5, 9, 1), (300000, 9, 1),
+                                   (12, 40, 6), (2, 4097, 1), (1, 65536, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_every_kernel_at_its_borders(shape, sigmoid, gc):
+    run(gc, shape, sigmoid)
+
+
+def test_thousands_of_calls_in_a_row(gc):
+    """Tiles hand states on through words that carry the call's number, of which there are 4095 before they start again;
+    calls of other sizes, which need more words, come between."""
+    small = [gc.createRaw(list(a.shape), a) for a in (gates(1, (1, 300, 65), True), data(2, 1, 300, 65))]
+    narrow = [gc.createRaw(list(a.shape), a) for a in (gates(3, (1, 9000, 2), True), data(4, 1, 9000, 2))]
+    large = [gc.createRaw(list(a.shape), a) for a in (gates(5, (2, 3000, 130), True), data(6, 2, 3000, 130))]
+    op = gc.gatedRecurrence(1)
+    want = {}
+    for i in range(4300):
+        for name, raw in (("small", small), ("narrow", narrow if i % 50 == 0 else None), ("large", large if i in (100, 4200) else None)):
+            if raw is None:
+                continue
+            out, final = op.calculateOutput(*raw)
+            if i < 3 or i % 500 == 0 or i in (100, 4200) or 4090 < i < 4100:
+                got = out.toArray()
+                want.setdefault(name, got)
+                assert_bits_equal(got, want[name], f"call {i}, {name}")
+            out.release(); final.release()
+
+
+def test_two_threads_at_once(gc):
+    """Calls from several threads follow one another: each gets its own results."""
+    import threading
+    made = []
+    for k in range(2):
+        shape = (2, 2000 + 500 * k, 65)
+        raw = [gc.createRaw(list(a.shape), a) for a in (gates(k, shape, True), data(k + 5, *shape))]
+        made.append((raw, gc.gatedRecurrence(1).calculateOutput(*raw)[0].toArray()))
+    errors = []
+
+    def work(k):
+        raw, want = made[k]
+        h = [t.storeReference for t in raw]
+        out = outs[k]
+        for _ in range(60):
+            if gc.lib.kth_gated_recurrence_forward(h[0], h[1], abi.shape_array(raw[0].shape), 3, 1, 1, 0, out.storeReference, 0) != 0:
+                errors.append(k)
+
+    outs = [gc.createRaw(m[0][0].shape) for m in made]
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads: t.start()
+    for t in threads: t.join()
+    assert not errors
+    for k in range(2):
+        assert_bits_equal(outs[k].toArray(), made[k][1], f"thread {k}")
+
+
 def test_refusals(gc):
     g, x, state = gc.createRaw([2, 4, 3], data(1, 2, 4, 3)), gc.createRaw([2, 4, 3], data(2, 2, 4, 3)), gc.createRaw([2, 3], data(3, 2, 3))
     out, final, short = gc.createRawFill([2, 4, 3], 9.0), gc.createRawFill([2, 3], 9.0), gc.createRaw([5])
