@@ -133,10 +133,11 @@ struct State {
     int*          host_index_flag_device = nullptr;
     IndexUse      index_use;
 
-    // what the tiles of a recurrence hand on through (kth_recurrence.hip): words, the last launch's tag, tickets drawn so far
+    // what the tiles of a recurrence hand on through (kth_recurrence.hip): words, the last launch's tag
     uint64_t* scan = nullptr;
     uint64_t  scan_words = 0;
-    uint32_t  scan_tag = 0, scan_tickets = 0;
+    uint32_t  scan_tag = 0;
+    static constexpr int kScanLost = 16;        // the int behind host_index_flag that a recurrence sets if a wait was given up
 
     std::vector<hipEvent_t> laps;           // kth_timer_lap events not yet read by kth_timer_laps
 

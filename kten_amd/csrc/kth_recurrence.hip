@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 // is read once. A step is the map K -> a K + u of the state, so a run of steps is one pair (A, H): waves exchange theirs
 // through LDS, tiles through memory.
 //
-// Tiles are drawn by ticket, earliest steps of all channels first. A tile only waits for tiles of earlier steps, which
-// have lower tickets and thus run already or have ended: every wait ends. Tile p reads the pairs of the tiles since the
+// Tiles are drawn from a counter, earliest steps of all channels first. A tile only waits for tiles of earlier steps, which
+// are drawn before it and thus run already or have ended: every wait ends. Tile p reads the pairs of the tiles since the
 // last multiple of kSuper before it, and the state that the tile before that multiple published: at most kSuper - 1 pairs
 // and one state, always composed in the same order, so the bits do not depend on who came first.
 //
@@ -156,9 +156,16 @@ __device__ __forceinline__ void publish(uint64_t* word, double v, uint32_t tag) 
     const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v)) + (1ull << (kTagBits - 1));
     __hip_atomic_store(word, (bits & ~static_cast<uint64_t>(kTags)) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ double await(const uint64_t* word, uint32_t tag) {
+// Waits for a word of an earlier tile. Should it not come within kMostPolls (seconds; a tile takes microseconds) the wave goes
+// on with NaN and leaves a mark for the host, which reports it at its next wait for the stream: no wait is endless.
+constexpr uint32_t kMostPolls = 1u << 22;
+__device__ __forceinline__ double await(const uint64_t* word, uint32_t tag, int* lost) {
     uint64_t bits = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    while ((bits & kTags) != tag) {
+    for (uint32_t polls = 0; (bits & kTags) != tag; polls++) {
+        if (polls == kMostPolls) {
+            __hip_atomic_store(lost, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            return __builtin_nan("");
+        }
         __builtin_amdgcn_s_sleep(1);
         bits = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -175,8 +182,8 @@ struct TilePlan {
     uint32_t cw, tw;                 // waves of a workgroup across channels and along steps
     uint32_t padded;                 // groups x cw x 64: channels with their padding
     uint32_t tag;
-    uint32_t ticket_base;
-    uint32_t* tickets;
+    uint32_t* tickets;               // this launch's counter
+    int*      lost;                  // the host's word for a wait that was given up
     uint64_t* pairs;                 // [tiles][padded][2]
     uint64_t* states;                // [tiles / kSuper][padded]
     FastDiv  group_div, col_div;
@@ -199,7 +206,7 @@ struct TilePlace {
 
 __device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* lds_ticket) {
     TilePlace w;
-    if (threadIdx.x == 0) *lds_ticket = pl.tiles > 1 ? atomicAdd(pl.tickets, 1u) - pl.ticket_base : blockIdx.x;
+    if (threadIdx.x == 0) *lds_ticket = pl.tiles > 1 ? atomicAdd(pl.tickets, 1u) : blockIdx.x;
     __syncthreads();
     const uint32_t ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -246,11 +253,11 @@ __device__ __forceinline__ double state_before(const TilePlan& pl, const TilePla
             Pair p{1.0, 0.0};
             for (uint32_t i = from; i < to; i++) {
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + i) * pl.padded + w.slot) * 2;
-                const double a = await(word, pl.tag), h = await(word + 1, pl.tag);
+                const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
                 p = Pair{a * p.A, advance(a, h, p.H)};
             }
             before[w.twi * width + at] = p;
-            state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag);
+            state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag, pl.lost);
             __syncthreads();
             for (uint32_t i = 0; i < pl.tw; i++) { const Pair q = before[i * width + at]; state = advance(q.A, q.H, state); }
         }
@@ -404,8 +411,9 @@ struct NarrowPlan {
     uint32_t pieces;                 // of kSub steps, of a row in a workgroup
     uint32_t tile_steps, tiles;
     uint32_t channels;               // outer x inner
-    uint32_t tag, ticket_base;
-    uint32_t* tickets;
+    uint32_t tag;
+    uint32_t* tickets;               // this launch's counter
+    int*      lost;                  // the host's word for a wait that was given up
     uint64_t* pairs;                 // [tiles][channels][2]
     uint64_t* states;                // [tiles / kSuper][channels]
     FastDiv  inner_div, row_div, outer_div, piece_div;     // row_div divides by the floats of a row of this workgroup
@@ -422,7 +430,7 @@ struct NarrowPlace {
 __device__ __forceinline__ bool place_narrow(const NarrowPlan& pl, uint32_t* lds_ticket, NarrowPlace& w) {
     uint32_t ticket = blockIdx.x;
     if (pl.tiles > 1) {
-        if (threadIdx.x == 0) *lds_ticket = atomicAdd(pl.tickets, 1u) - pl.ticket_base;
+        if (threadIdx.x == 0) *lds_ticket = atomicAdd(pl.tickets, 1u);
         __syncthreads();
         ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
         if (ticket >= pl.tiles * pl.outer) return false;
@@ -488,13 +496,13 @@ __device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, cons
             for (uint32_t i = threadIdx.x; i < many * pl.inner; i += kNarrowThreads) {
                 const uint32_t t = divide(i, pl.inner_div);
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + t) * pl.channels + w.o0 * pl.inner + (i - t * pl.inner)) * 2;
-                const double a = await(word, pl.tag), h = await(word + 1, pl.tag);
+                const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
                 handed[i] = Pair{a, h};
             }
             __syncthreads();
             if (threadIdx.x < pl.inner) {
                 const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
-                double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.tag);
+                double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.tag, pl.lost);
                 for (uint32_t t = 0; t < many; t++) { const Pair p = handed[t * pl.inner + threadIdx.x]; s = advance(p.A, p.H, s); }
                 carried[threadIdx.x] = s;
                 if (many + 1 == kSuper && w.tile + 1 < pl.tiles)
@@ -655,9 +663,9 @@ Path path_of(const ScanShape& sh, bool forward) {
 }
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
-// one stream, and each has a tag and a range of tickets of its own.
-int take_words(const char* what, uint64_t words, uint32_t tickets, uint32_t* tag, uint32_t* ticket_base, uint32_t** counter, uint64_t** first) {
-    constexpr uint64_t kHead = 64;                           // the ticket counter, on cache lines of its own
+// one stream, and each has a tag and a counter of its own.
+int take_words(const char* what, uint64_t words, uint32_t* tag, uint32_t** counter, uint64_t** first, int** lost) {
+    constexpr uint64_t kHead = (kTags + 1) / 2;              // every tag's counter
     State& s = state();
     words += kHead;
     if (words > s.scan_words || s.scan_tag == kTags) {
@@ -675,14 +683,13 @@ int take_words(const char* what, uint64_t words, uint32_t tickets, uint32_t* tag
         }
         for (uint64_t at = 0; at < s.scan_words; at += 1ull << 29)
             launch_fill(reinterpret_cast<float*>(s.scan + at), 2 * std::min<uint64_t>(s.scan_words - at, 1ull << 29), 0.0f);
-        s.scan_tag = 0; s.scan_tickets = 0;
+        s.scan_tag = 0;
     }
     s.scan_tag += 1;
     *tag = s.scan_tag;
-    *ticket_base = s.scan_tickets;
-    s.scan_tickets += tickets;                               // (wraps, as the counter does)
-    *counter = reinterpret_cast<uint32_t*>(s.scan);
+    *counter = reinterpret_cast<uint32_t*>(s.scan) + s.scan_tag;
     *first = s.scan + kHead;
+    *lost = s.host_index_flag_device + State::kScanLost;
     return KTH_OK;
 }
 
@@ -698,8 +705,7 @@ int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     pl.col_div = make_div(pl.col_blocks);
     if (pl.tiles > 1) {
         const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.padded * 2;
-        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded, pl.tiles * pl.groups, &pl.tag, &pl.ticket_base,
-                                &pl.tickets, &pl.pairs)) return rc;
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded, &pl.tag, &pl.tickets, &pl.pairs, &pl.lost)) return rc;
         pl.states = pl.pairs + pairs;
     }
     *out = pl;
@@ -723,20 +729,12 @@ int plan_narrow(const char* what, const ScanShape& sh, NarrowPlan* out, uint32_t
     *grid = pl.tiles > 1 ? pl.tiles * sh.outer : (sh.outer - 1) / pl.rows + 1;
     if (pl.tiles > 1) {
         const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.channels * 2;
-        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.channels, *grid, &pl.tag, &pl.ticket_base, &pl.tickets,
-                                &pl.pairs)) return rc;
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.channels, &pl.tag, &pl.tickets, &pl.pairs, &pl.lost))
+            return rc;
         pl.states = pl.pairs + pairs;
     }
     *out = pl;
     return KTH_OK;
-}
-
-// (as KTH_LAUNCH_CHECK) A launch that failed drew no tickets: the next one starts from cleared words.
-int tiles_launched(const char* what) {
-    const hipError_t e = hipGetLastError();
-    if (e == hipSuccess) return KTH_OK;
-    state().scan_tag = kTags;
-    return fail(KTH_E_DEVICE, "launch of %s failed: %s", what, hipGetErrorString(e));
 }
 
 uint32_t tile_lds(const TilePlan& pl) { return 2 * pl.tw * pl.cw * 64 * static_cast<uint32_t>(sizeof(Pair)); }
@@ -786,7 +784,8 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         LaunchScope scope("recurrence_forward_narrow_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
         auto* kernel = sigmoid ? recurrence_forward_narrow_kernel<true> : recurrence_forward_narrow_kernel<false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
-        return tiles_launched("gated_recurrence_forward");
+        KTH_LAUNCH_CHECK("gated_recurrence_forward");
+        return KTH_OK;
     }
     if (path == Path::tiles) {
         constexpr int L = 32;
@@ -798,7 +797,8 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         auto* kernel = sigmoid ? (lines ? recurrence_forward_tiles_kernel<true, true, L> : recurrence_forward_tiles_kernel<true, false, L>)
                                : (lines ? recurrence_forward_tiles_kernel<false, true, L> : recurrence_forward_tiles_kernel<false, false, L>);
         hipLaunchKernelGGL(kernel, grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
-        return tiles_launched("gated_recurrence_forward");
+        KTH_LAUNCH_CHECK("gated_recurrence_forward");
+        return KTH_OK;
     }
     LaunchScope scope("recurrence_forward_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);
@@ -836,7 +836,8 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
         auto* kernel = sigmoid ? recurrence_backward_narrow_kernel<true> : recurrence_backward_narrow_kernel<false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
                            ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
-        return tiles_launched("gated_recurrence_backward");
+        KTH_LAUNCH_CHECK("gated_recurrence_backward");
+        return KTH_OK;
     }
     if (path == Path::tiles) {
         constexpr int L = 16;
@@ -849,7 +850,8 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
                                : (lines ? recurrence_backward_tiles_kernel<false, true, L> : recurrence_backward_tiles_kernel<false, false, L>);
         hipLaunchKernelGGL(kernel, grid, block, tile_lds(pl), state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
                            ops[5].ptr, ops[6].ptr, ops[7].ptr, ops[8].ptr, pl);
-        return tiles_launched("gated_recurrence_backward");
+        KTH_LAUNCH_CHECK("gated_recurrence_backward");
+        return KTH_OK;
     }
     LaunchScope scope("recurrence_backward_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);

@@ -315,6 +315,10 @@ void events_for_launch(hipEvent_t* begin, hipEvent_t* end) {
 
 int report_deferred_index_error() {
     State& s = state();
+    if (s.host_index_flag && s.host_index_flag[State::kScanLost] != 0) {
+        s.host_index_flag[State::kScanLost] = 0;
+        return fail(KTH_E_DEVICE, "a recurrence gave up waiting for the state of earlier steps: its results are not valid");
+    }
     if (s.index_check_immediate || !s.deferred_index_flag) return KTH_OK;
     int host_flag = 0;
     KTH_HIP(hipMemcpyAsync(&host_flag, s.deferred_index_flag, 4, hipMemcpyDeviceToHost, s.stream));
@@ -380,6 +384,7 @@ static int bring_up(int device) {
     KTH_HIP(hipHostGetDevicePointer(&dev, host, 0));
     s.host_index_flag_device = static_cast<int*>(dev);
     *s.host_index_flag = 0;
+    s.host_index_flag[State::kScanLost] = 0;
     return KTH_OK;
 }
 
