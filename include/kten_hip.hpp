@@ -229,6 +229,54 @@ public:
         int axis_; float momentum_, epsilon_; bool training_; HipTensorOperations* ops_;
     };
     BatchNorm batchNorm(int axis, float momentum, float epsilon, bool training) { return BatchNorm(axis, momentum, epsilon, training, this); }
+
+    // The layers over sequences (no counterpart in the reference), shaped like batchNorm. Absent tensors are null.
+    // Layer normalisation over the dims from `axis` on; the statistics have the shape of the dims before it.
+    struct LayerNormOutputs { Raw output, currentMean, currentStd; };
+    struct LayerNormGrads { Raw gradIn, gradGamma, gradBeta; };
+    class LayerNorm {
+    public:
+        LayerNorm(int axis, float epsilon, HipTensorOperations* ops) : axis_(axis), epsilon_(epsilon), ops_(ops) {}
+        LayerNormOutputs calculateOutput(const Raw& input, const Raw& gamma, const Raw& beta);
+        LayerNormGrads calculateGrads(const Raw& input, const Raw& gamma, const Raw& gradOut, bool inRequiresGrad, bool gammaRequiresGrad,
+                                      bool betaRequiresGrad);
+    private:
+        int axis_; float epsilon_; HipTensorOperations* ops_;
+    };
+    LayerNorm layerNorm(int axis, float epsilon) { return LayerNorm(axis, epsilon, this); }
+
+    // Dropout: p, seed and offset say which values are kept, so the input's gradient is the same call on the output's; a
+    // layer that is called again advances its offset by (elements + 3) / 4.
+    class Dropout {
+    public:
+        Dropout(double p, uint64_t seed, uint64_t offset, HipTensorOperations* ops) : p_(p), seed_(seed), offset_(offset), ops_(ops) {
+            if (!(p >= 0.0 && p <= 1.0)) throw std::invalid_argument("dropout probability outside [0, 1]");
+        }
+        Raw calculateOutput(const Raw& input, const Raw& residual = nullptr);
+        Raw calculateGrad(const Raw& gradOut) { return calculateOutput(gradOut); }
+    private:
+        double p_; uint64_t seed_, offset_; HipTensorOperations* ops_;
+    };
+    Dropout dropout(double p, uint64_t seed, uint64_t offset = 0) { return Dropout(p, seed, offset, this); }
+
+    // The gated linear recurrence along `axis`: with sigmoidGate the step's factor is s = sigmoid(gate) and its input
+    // (1 - s) input, else they are gate and input themselves. The state has the shape of the other dims.
+    struct RecurrenceOutputs { Raw output, finalState; };
+    struct RecurrenceGrads { Raw gradGate, gradIn, gradInitial; };
+    class GatedRecurrence {
+    public:
+        GatedRecurrence(int axis, bool sigmoidGate, HipTensorOperations* ops)
+            : axis_(axis), mode_(sigmoidGate ? KTH_GATE_SIGMOID : KTH_GATE_GIVEN), ops_(ops) {}
+        RecurrenceOutputs calculateOutput(const Raw& gate, const Raw& input, const Raw& initial);
+        Raw step(const Raw& gate, const Raw& input, const Raw& state);          // `state` is updated in place
+        RecurrenceGrads calculateGrads(const Raw& gate, const Raw& input, const Raw& initial, const Raw& output, const Raw& gradOut,
+                                       const Raw& gradFinal, bool gateRequiresGrad, bool inRequiresGrad, bool initialRequiresGrad);
+    private:
+        Shape stateShape(const Raw& gate, const Raw& input, const Raw& initial, int* axis) const;
+        int axis_, mode_; HipTensorOperations* ops_;
+    };
+    GatedRecurrence gatedRecurrence(int axis, bool sigmoidGate = true) { return GatedRecurrence(axis, sigmoidGate, this); }
+
     void release(const Raw& t);                                     // :22
     void incrementRef(const Raw& t);                                // :28
     void markSurviveGC(const Raw& t);                               // :30-33 / OCLTensorOperations.kt:96-98
@@ -264,6 +312,7 @@ public:
 private:
     friend class HipRawTensor;
     void collect(const Raw& t) { if (collecting_) instances_.push_back(t); }
+    static uint64_t handleOf(const Raw& t);                         // 0 for an absent tensor
     bool collecting_ = false;
     std::vector<Raw> instances_, survivors_;
 };
@@ -699,6 +748,103 @@ inline HipTensorOperations::BatchNormGrads HipTensorOperations::BatchNorm::calcu
     check(kth_batch_norm_backward(input->storeReference, input->shape.data(), input->dimensions(), axis, training_ ? 1 : 0, epsilon_,
                                   h(runningMean), h(runningVar), h(currentMean), h(currentStd), h(gamma), gradOut->storeReference,
                                   h(r.gradIn), h(r.gradGamma), h(r.gradBeta)));
+    return r;
+}
+
+// The layers over sequences: a handle of 0 for what is absent, the element counts checked before anything is allocated.
+inline uint64_t HipTensorOperations::handleOf(const Raw& t) {
+    if (!t) return 0;
+    t->live();
+    return t->storeReference;
+}
+namespace detail {
+inline void requireSize(const char* what, const Raw& t, int64_t n) {
+    if (t && toStoreSize(t->shape) != n)
+        throw std::invalid_argument(std::string(what) + " must hold " + std::to_string(n) + " values, got shape " + to_string(t->shape));
+}
+inline Shape orOne(Shape s) { return s.empty() ? Shape{1} : s; }
+}  // namespace detail
+
+inline HipTensorOperations::LayerNormOutputs HipTensorOperations::LayerNorm::calculateOutput(const Raw& input, const Raw& gamma, const Raw& beta) {
+    const uint64_t in = handleOf(input), g = handleOf(gamma), b = handleOf(beta);
+    const int axis = normalizeAxis(input->shape, axis_);
+    const Shape weights(input->shape.begin() + axis, input->shape.end()), rows(input->shape.begin(), input->shape.begin() + axis);
+    detail::requireSize("Gamma of a layer normalization", gamma, toStoreSize(weights));
+    detail::requireSize("Beta of a layer normalization", beta, toStoreSize(weights));
+    LayerNormOutputs r{ops_->createRaw(input->shape), ops_->createRaw(detail::orOne(rows)), ops_->createRaw(detail::orOne(rows))};
+    check(kth_layer_norm_forward(in, input->shape.data(), input->dimensions(), axis, epsilon_, g, b, r.output->storeReference,
+                                 r.currentMean->storeReference, r.currentStd->storeReference));
+    return r;
+}
+inline HipTensorOperations::LayerNormGrads HipTensorOperations::LayerNorm::calculateGrads(
+        const Raw& input, const Raw& gamma, const Raw& gradOut, bool inRequiresGrad, bool gammaRequiresGrad, bool betaRequiresGrad) {
+    LayerNormGrads r{};
+    if (!inRequiresGrad && !gammaRequiresGrad && !betaRequiresGrad) return r;
+    const uint64_t in = handleOf(input), g = handleOf(gamma), go = handleOf(gradOut);
+    const int axis = normalizeAxis(input->shape, axis_);
+    const Shape weights(input->shape.begin() + axis, input->shape.end());
+    detail::requireSize("Gamma of a layer normalization", gamma, toStoreSize(weights));
+    detail::requireSize("The gradient of a layer normalization's output", gradOut, toStoreSize(input->shape));
+    if (inRequiresGrad) r.gradIn = ops_->createRaw(input->shape);
+    if (gammaRequiresGrad) r.gradGamma = ops_->createRaw(weights);
+    if (betaRequiresGrad) r.gradBeta = ops_->createRaw(weights);
+    check(kth_layer_norm_backward(in, input->shape.data(), input->dimensions(), axis, epsilon_, g, go, handleOf(r.gradIn),
+                                  handleOf(r.gradGamma), handleOf(r.gradBeta)));
+    return r;
+}
+inline Raw HipTensorOperations::Dropout::calculateOutput(const Raw& input, const Raw& residual) {
+    const uint64_t in = handleOf(input), add = handleOf(residual);
+    detail::requireSize("The residual of a dropout", residual, toStoreSize(input->shape));
+    Raw r = ops_->createRaw(input->shape);
+    check(kth_dropout(in, static_cast<uint64_t>(toStoreSize(input->shape)), p_, seed_, offset_, add, r->storeReference));
+    return r;
+}
+inline Shape HipTensorOperations::GatedRecurrence::stateShape(const Raw& gate, const Raw& input, const Raw& initial, int* axis) const {
+    if (gate->shape != input->shape)
+        throw std::invalid_argument("Gate and input of a recurrence must have the same shape, got " + to_string(gate->shape) + " and " +
+                                    to_string(input->shape));
+    *axis = normalizeAxis(input->shape, axis_);
+    Shape state = input->shape;
+    state.erase(state.begin() + *axis);
+    detail::requireSize("The initial state of a recurrence", initial, toStoreSize(state));
+    return detail::orOne(state);
+}
+inline HipTensorOperations::RecurrenceOutputs HipTensorOperations::GatedRecurrence::calculateOutput(const Raw& gate, const Raw& input,
+                                                                                                    const Raw& initial) {
+    const uint64_t g = handleOf(gate), in = handleOf(input), h0 = handleOf(initial);
+    int axis = 0;
+    const Shape state = stateShape(gate, input, initial, &axis);
+    RecurrenceOutputs r{ops_->createRaw(input->shape), ops_->createRaw(state)};
+    check(kth_gated_recurrence_forward(g, in, input->shape.data(), input->dimensions(), axis, mode_, h0, r.output->storeReference,
+                                       r.finalState->storeReference));
+    return r;
+}
+inline Raw HipTensorOperations::GatedRecurrence::step(const Raw& gate, const Raw& input, const Raw& state) {
+    const uint64_t g = handleOf(gate), in = handleOf(input), h = handleOf(state);
+    int axis = 0;
+    stateShape(gate, input, state, &axis);
+    Raw r = ops_->createRaw(input->shape);
+    check(kth_gated_recurrence_forward(g, in, input->shape.data(), input->dimensions(), axis, mode_, h, r->storeReference, h));
+    return r;
+}
+inline HipTensorOperations::RecurrenceGrads HipTensorOperations::GatedRecurrence::calculateGrads(
+        const Raw& gate, const Raw& input, const Raw& initial, const Raw& output, const Raw& gradOut, const Raw& gradFinal,
+        bool gateRequiresGrad, bool inRequiresGrad, bool initialRequiresGrad) {
+    RecurrenceGrads r{};
+    if (!gateRequiresGrad && !inRequiresGrad && !initialRequiresGrad) return r;
+    const uint64_t g = handleOf(gate), in = handleOf(input), h0 = handleOf(initial), out = handleOf(output),
+                   go = handleOf(gradOut), gf = handleOf(gradFinal);
+    int axis = 0;
+    const Shape state = stateShape(gate, input, initial, &axis);
+    const int64_t n = toStoreSize(gate->shape);
+    detail::requireSize("The gradient of a recurrence's output", gradOut, n);
+    detail::requireSize("The output of a recurrence", output, n);
+    detail::requireSize("The gradient of a recurrence's last state", gradFinal, toStoreSize(state));
+    if (gateRequiresGrad) r.gradGate = ops_->createRaw(gate->shape);
+    if (inRequiresGrad) r.gradIn = ops_->createRaw(gate->shape);
+    if (initialRequiresGrad) r.gradInitial = ops_->createRaw(state);
+    check(kth_gated_recurrence_backward(g, in, gate->shape.data(), gate->dimensions(), axis, mode_, h0, out, go, gf, handleOf(r.gradGate),
+                                        handleOf(r.gradIn), handleOf(r.gradInitial)));
     return r;
 }
 inline void HipTensorOperations::release(const Raw& t) { t->release(); }
