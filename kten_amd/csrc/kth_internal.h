@@ -200,6 +200,18 @@ struct Operand {
 // the inputs are owed is launched, and what the results are owed dropped or launched.
 int resolve_operands(const char* what, Operand* ops, int count, std::initializer_list<std::pair<int, int>> allowed, int size_code = KTH_E_SHAPE);
 
+// Makes the library's device the calling thread's current one for a while: memory is allocated on the current device, and
+// a host's thread may have chosen another, or none yet.
+class OnDevice {
+public:
+    OnDevice() { if (hipGetDevice(&before_) != hipSuccess || before_ == state().device) before_ = -1; else (void)hipSetDevice(state().device); }
+    ~OnDevice() { if (before_ >= 0) (void)hipSetDevice(before_); }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+private:
+    int before_ = -1;
+};
+
 // Pool-backed raw device memory for kernels' own workspaces (partials of two-pass
 // reductions). Stream-ordered: a workspace returned to the pool may be reused by a
 // later launch because every launch is on the one in-order stream.

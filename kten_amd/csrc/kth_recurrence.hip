@@ -12,6 +12,7 @@
 #include "kth_internal.h"
 
 #include <algorithm>
+#include <climits>
 
 using namespace kth;
 
@@ -175,6 +176,28 @@ __device__ __forceinline__ double await(const uint64_t* word, uint32_t tag, int*
 // A state that is zero stays so, whatever the product of the gates (which may have overflowed).
 __device__ __forceinline__ double advance(double A, double H, double state) { return state == 0.0 ? H : fma(A, state, H); }
 
+// A product of gates none of which is zero does not become zero either (an infinite state stays infinite under any decay):
+// below the normal range it stays at that range's end, which moves no finite state that fp32 can hold.
+constexpr double kLeast = 2.2250738585072014e-308;       // 2^-1022
+__device__ __forceinline__ double product(double later, double earlier) {
+    const double r = later * earlier;
+    return fabs(r) < kLeast && later != 0.0 && earlier != 0.0 ? copysign(kLeast, r) : r;
+}
+// The same for the steps of one run, whose gates are multiplied to A one by one. `least` is kept by an instruction a step and
+// without a branch (a look at the gates where A is that small makes the compiler keep twice the registers: 48 to 78 us for
+// [8,2048,1024]); it tells whether a gate was zero, which is -0 where gates are packed logits, the smallest of all integers.
+template <bool SIGMOID>
+struct Least {
+    float abs = INFINITY;
+    int   bits = INT_MAX;
+    __device__ __forceinline__ void take(float v) {
+        if (SIGMOID) bits = min(bits, __float_as_int(v)); else abs = fminf(abs, fabsf(v));
+    }
+    __device__ __forceinline__ double keep(double A) const {
+        return fabs(A) < kLeast && (SIGMOID ? bits != INT_MIN : abs != 0.0f) ? copysign(kLeast, A) : A;
+    }
+};
+
 struct TilePlan {
     uint32_t steps, inner;
     uint32_t col_blocks, groups;     // workgroups across one outer index; across all channels (outer x col_blocks)
@@ -239,7 +262,7 @@ __device__ __forceinline__ double state_before(const TilePlan& pl, const TilePla
             Pair total = lds[at];
             for (uint32_t i = 1; i < pl.tw; i++) {
                 const Pair p = lds[i * width + at];
-                total = Pair{p.A * total.A, advance(p.A, p.H, total.H)};
+                total = Pair{product(p.A, total.A), advance(p.A, p.H, total.H)};
             }
             if (w.tile == 0) total = Pair{0.0, advance(total.A, total.H, initial)};     // nobody else reads `initial`
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
@@ -254,7 +277,7 @@ __device__ __forceinline__ double state_before(const TilePlan& pl, const TilePla
             for (uint32_t i = from; i < to; i++) {
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + i) * pl.padded + w.slot) * 2;
                 const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
-                p = Pair{a * p.A, advance(a, h, p.H)};
+                p = Pair{product(a, p.A), advance(a, h, p.H)};
             }
             before[w.twi * width + at] = p;
             state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag, pl.lost);
@@ -299,6 +322,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
         if (t0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; u[k] = 0.0f; }
     const double start = w.tile == 0 && initial ? static_cast<double>(initial[w.first_state]) : 0.0;
     double A = 1.0, H = 0.0;
+    Least<SIGMOID> least;
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (SIGMOID) {
@@ -308,11 +332,12 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
         const double a = gate_a<SIGMOID>(v[k]);
         H = fma(a, H, static_cast<double>(u[k]));
         A *= a;
+        least.take(v[k]);
         KTH_STEPS_APART(k);
     }
 #pragma unroll
     for (int k = 0; k < L; k++) { forget(v[k]); forget(u[k]); }
-    double h = state_before(pl, w, A, H, start, lds);
+    double h = state_before(pl, w, least.keep(A), H, start, lds);
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (t0 + k < pl.steps) {
@@ -350,12 +375,14 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
         if (q0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; g[k] = 0.0f; }
     const double start = w.tile == 0 && grad_final ? static_cast<double>(grad_final[w.first_state]) : 0.0;
     double A = 1.0, H = 0.0;
+    Least<SIGMOID> least;
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (SIGMOID) v[k] = pack_gate<SIGMOID>(v[k]);
         const double a = gate_a<SIGMOID>(v[k]);
         H = a * (static_cast<double>(g[k]) + H);
         A *= a;
+        least.take(v[k]);
         KTH_STEPS_APART(k);
     }
 #pragma unroll
@@ -376,7 +403,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
             for (int k = 0; k < L; k++) if (q0 + k + 1 == pl.steps) before[k] = h0;
         }
     }
-    double K = state_before(pl, w, A, H, start, lds);
+    double K = state_before(pl, w, least.keep(A), H, start, lds);
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (q0 + k < pl.steps) {
@@ -477,7 +504,7 @@ __device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, cons
         __syncthreads();
         if (w.works && w.j >= d) {
             const Pair p = pair[threadIdx.x - d * pl.inner];
-            mine = Pair{mine.A * p.A, advance(mine.A, mine.H, p.H)};
+            mine = Pair{product(mine.A, p.A), advance(mine.A, mine.H, p.H)};
         }
         __syncthreads();
     }
@@ -546,6 +573,7 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kern
     const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
     const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
     double A = 1.0, H = 0.0;
+    Least<SIGMOID> least;
     for (uint32_t k = 0; k < count; k++) {
         const uint32_t i = base + k * pl.inner;
         const float v = pack_gate<SIGMOID>(sh.a[i]);
@@ -554,8 +582,9 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kern
         const double a = gate_a<SIGMOID>(v);
         H = fma(a, H, static_cast<double>(u));
         A *= a;
+        least.take(v);
     }
-    double h = narrow_state_before(pl, w, A, H, start, sh.pair, sh.handed, sh.carried);
+    double h = narrow_state_before(pl, w, least.keep(A), H, start, sh.pair, sh.handed, sh.carried);
     for (uint32_t k = 0; k < count; k++) {
         const uint32_t i = base + k * pl.inner;
         h = fma(gate_a<SIGMOID>(sh.a[i]), h, static_cast<double>(sh.b[i]));
@@ -592,6 +621,7 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
     const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
     const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
     double A = 1.0, H = 0.0;
+    Least<SIGMOID> least;
     float v[kSub], g[kSub];
 #pragma unroll
     for (uint32_t k = 0; k < kSub; k++) {
@@ -602,9 +632,10 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
             const double a = gate_a<SIGMOID>(v[k]);
             H = a * (static_cast<double>(g[k]) + H);
             A *= a;
+            least.take(v[k]);
         }
     }
-    double K = narrow_state_before(pl, w, A, H, start, sh.pair, sh.handed, sh.carried);
+    double K = narrow_state_before(pl, w, least.keep(A), H, start, sh.pair, sh.handed, sh.carried);
     __syncthreads();                                                   // gate and grad_out are in registers: their LDS is free
     if (grad_gate) {                                                   // (without it out and in need not be given)
 #pragma unroll 8
@@ -673,6 +704,7 @@ int take_words(const char* what, uint64_t words, uint32_t* tag, uint32_t** count
             KTH_HIP(hipStreamSynchronize(s.stream));
             if (s.scan) KTH_HIP(hipFree(s.scan));
             s.scan = nullptr; s.scan_words = 0;
+            const OnDevice here;
             void* p = nullptr;
             if (hipMalloc(&p, words * 8) != hipSuccess) {
                 (void)hipGetLastError();

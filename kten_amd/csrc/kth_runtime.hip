@@ -248,6 +248,7 @@ static float* pool_take(uint64_t cap) {
         trim_pool();
         if (s.live_bytes + cap > budget) return nullptr;
     }
+    const OnDevice here;
     void* p = nullptr;
     if (hipMalloc(&p, cap) != hipSuccess) {
         (void)hipGetLastError();

@@ -123,6 +123,37 @@ def test_nan_stays_in_its_channel_and_after_its_step(shape, gc):
     assert np.isnan(got[0, t - 1:, 1]).all()         # 0 x NaN: the formula's result
 
 
+@pytest.mark.parametrize("shape", [(2, 8, 70), (1, 4000, 70), (1, 4000, 3)], ids=lambda s: "x".join(map(str, s)))
+def test_infinite_gate_and_infinite_input(shape, gc):
+    """An infinite gate leaves its channel infinite or NaN from its step on, an infinite input infinite while the decay lasts
+    (0.5 here); steps before and other channels keep their bits."""
+    gate, x, state = np.full(shape, 0.5, np.float32), data(2, *shape), data(4, shape[0], shape[2])
+    op = gc.gatedRecurrence(1, False)
+    t = shape[1] // 2
+    clean = op.calculateOutput(*(gc.createRaw(list(a.shape), a) for a in (gate, x, state)))[0].toArray()
+    for which in (gate, x):
+        keep = which[0, t, 1]
+        which[0, t, 1] = np.inf
+        got = op.calculateOutput(*(gc.createRaw(list(a.shape), a) for a in (gate, x, state)))[0].toArray()
+        if which is x:
+            assert (got[0, t:, 1] == np.inf).all()
+        else:
+            assert np.isinf(got[0, t, 1]) and not np.isfinite(got[0, t:, 1]).any()
+        got[0, t:, 1] = clean[0, t:, 1]
+        assert_bits_equal(got, clean, "the other channels, and the steps before")
+        which[0, t, 1] = keep
+    # the same towards the first step for an infinite gradient
+    zero = np.zeros(shape, np.float32)
+    zero[0, t, 1] = np.inf
+    grad = op.calculateGrads(*(gc.createRaw(list(a.shape), a) for a in (gate, x, state, clean, zero)))
+    want = np.zeros(shape, np.float32)
+    want[0, :t + 1, 1] = np.inf
+    assert_bits_equal(grad[1].toArray(), want, "gradIn")
+    want = np.zeros(state.shape, np.float32)
+    want[0, 1] = np.inf
+    assert_bits_equal(grad[2].toArray().reshape(state.shape), want, "gradInitial")
+
+
 def test_axes(gc):
     full = data(1, 4, 5, 6, 7)
     gate, go = gates(2, full.shape, True), data(3, *full.shape)
