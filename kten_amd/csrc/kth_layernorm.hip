@@ -45,8 +45,9 @@ __device__ __forceinline__ double row_rstd(double v, double eps) {
     return s == 0.0 ? 0.0 : 1.0 / sqrt(s);
 }
 
-__device__ __forceinline__ float ln_forward(float x, double mean, float rstd, float gamma, float beta) {
-    return static_cast<float>(static_cast<double>(x) - mean) * rstd * gamma + beta;
+// (the product with rstd in f64: without epsilon it may be beyond fp32's range where a row's values are subnormal)
+__device__ __forceinline__ float ln_forward(float x, double mean, double rstd, float gamma, float beta) {
+    return static_cast<float>((static_cast<double>(x) - mean) * rstd) * gamma + beta;
 }
 
 // Sums of NS doubles over a workgroup of kBlock threads; every thread of wave 0 returns them.
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
 #pragma unroll
             for (int e = 0; e < 4; e++) forget(v[u][e]);
         const double mean = k + s[0] * sh.inv_cols;
-        const float rstd = static_cast<float>(row_rstd_fast(row_variance(s[0], s[1], sh.inv_cols), eps));
+        const double rstd = row_rstd_fast(row_variance(s[0], s[1], sh.inv_cols), eps);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float r[4];
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
         }
         if (lane == 0) {
             if (out_mean) out_mean[row] = static_cast<float>(mean);
-            if (out_std) out_std[row] = rstd;
+            if (out_std) out_std[row] = static_cast<float>(rstd);
         }
     }
 }
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(kBlock) void ln_apply_kernel(const float* x, const 
     const uint32_t first = seg * pl.seg_len;
     const uint32_t last = min(first + pl.seg_len, pl.sh.cols);
     const double mean = fwd[row].mean;
-    const float rstd = static_cast<float>(fwd[row].rstd);
+    const double rstd = fwd[row].rstd;
     for (uint32_t c = first + threadIdx.x * 4; c < last; c += kBlock * 4) {
         if (c + 4 <= last) {
             const v4f_any vx = *reinterpret_cast<const v4f_any*>(x + at + c);

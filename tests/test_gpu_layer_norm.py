@@ -93,6 +93,16 @@ def test_values_that_are_hard_on_the_statistics(cols, gc):
     assert not grads[0].toArray().any() and not grads[1].toArray().any()
 
 
+@pytest.mark.parametrize("cols", [5, 24, 900, 9000, 20000])
+def test_rows_of_subnormal_values_without_epsilon(cols, gc):
+    """1 / sqrt(var) is beyond fp32's range there, the normalised values are not."""
+    x = (np.random.default_rng(cols).integers(-200, 200, (3, cols)) * 2.0 ** -149).astype(np.float32)
+    gamma, beta = data(cols + 2, cols), data(cols + 3, cols)
+    out, mean, std = gc.layerNorm(1, 0.0).calculateOutput(*(gc.createRaw(list(a.shape), a) for a in (x, gamma, beta)))
+    ref.assert_within(out.toArray(), ref.layer_norm(x, gamma, beta, 0.0)[0], ref.layer_norm_bounds(x, gamma, beta, 0.0)[0], "output")
+    assert np.isinf(std.toArray()).all()
+
+
 @pytest.mark.parametrize("cols", [24, 900, 9000, 20000])
 def test_infinities_and_nan_stay_in_their_rows(cols, gc):
     x, go = data(cols, 6, cols), data(cols + 1, 6, cols)
