@@ -73,13 +73,17 @@ __device__ __forceinline__ void block_fold(double (&s)[NS], double* lds) {
 
 // G lanes hold a row, U float4s each (column (u G + lane) 4 + e), so that a pass reads its operands once: a row is summed,
 // its statistics are worked out by every lane, and the results are written from the registers. G = 4, 16 and 64 put
-// several rows into a wave or one, larger G a row into two waves or a workgroup.
-template <int G>
+// several rows into a wave or one, larger G a row into two waves or more. Forward, a row that waves share has a workgroup to
+// itself. Backward, a workgroup takes several rows at a time, because each leaves partial sums of the weights' gradients:
+// with 512 threads instead of 256 [8192,768] takes 21.4 us instead of 22.8, [2000,700] 12.3 instead of 14.6, [4096,512] 13.9
+// instead of 17.4; but two rows of 4096 columns, 256 lanes each, wait for each other ([16384,4096] 158 us instead of 153).
+template <int G, int T>
 struct RowGroup {
-    static constexpr int threads = G > 64 ? G : kBlock;      // a row that waves share has the workgroup to itself
+    static constexpr int threads = G > T ? G : T;              // of a workgroup
     static constexpr int groups = threads / G;                 // rows of a workgroup at a time
-    static constexpr int waves = G > 64 ? G / 64 : 0;          // that share a row
 };
+template <int G> using ForwardGroup = RowGroup<G, (G > 64 ? G : kBlock)>;
+template <int G, int U> using BackwardGroup = RowGroup<G, (G == 256 && U == 4 ? 256 : 512)>;
 
 // Lane sums of a double without LDS: both halves of the other lane's value by a register move (DPP inside 16 lanes, the
 // row swaps of permlane across them), then an f64 addition. Every step adds the same two values in every lane that takes
@@ -114,18 +118,18 @@ __device__ __forceinline__ double lanes_sum(double v) {
 }
 
 // Sums of NS doubles over the G lanes of a row; every lane gets them, added in the same order. `lds` holds two sets of
-// NS x waves doubles: sets alternate from row to row, so one barrier a row is enough.
-template <int G, int NS>
+// NS doubles a wave: sets alternate from row to row, so one barrier a row is enough.
+template <int G, int THREADS, int NS>
 __device__ __forceinline__ void row_fold(double (&s)[NS], double* lds, uint32_t& set) {
 #pragma unroll
     for (int i = 0; i < NS; i++) s[i] = lanes_sum<(G > 64 ? 64 : G)>(s[i]);
     if constexpr (G > 64) {
-        constexpr int waves = RowGroup<G>::waves;
-        double* mine = lds + set * NS * waves;
+        constexpr int waves = G / 64;
+        double* mine = lds + (set * (THREADS / G) + threadIdx.x / G) * NS * waves;
         set ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
-            for (int i = 0; i < NS; i++) mine[i * waves + (threadIdx.x >> 6)] = s[i];
+            for (int i = 0; i < NS; i++) mine[i * waves + (threadIdx.x % G >> 6)] = s[i];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NS; i++) s[i] = lanes_sum<waves>(mine[i * waves + threadIdx.x % waves]);
@@ -166,10 +170,10 @@ __device__ __forceinline__ void store4(float* p, uint32_t c, uint32_t cols, cons
 }
 
 template <int G, int U>
-__global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta,
+__global__ __launch_bounds__(ForwardGroup<G>::threads) void ln_forward_rows_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta,
                                                                                float* out, float* __restrict__ out_mean, float* __restrict__ out_std,
                                                                                Shape2 sh, double eps) {
-    __shared__ double lds[G > 64 ? 2 * 2 * RowGroup<G>::waves : 1];
+    __shared__ double lds[G > 64 ? 2 * 2 * G / 64 : 1];
     const uint32_t lane = threadIdx.x % G;
     uint32_t set = 0;
     float ga[U][4], be[U][4];
@@ -181,7 +185,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
         if (gamma) load4<false>(gamma, c, sh.cols, 1.0f, ga[u]);
         if (beta) load4<false>(beta, c, sh.cols, 0.0f, be[u]);
     }
-    for (uint32_t row = blockIdx.x * RowGroup<G>::groups + threadIdx.x / G; row < sh.rows; row += gridDim.x * RowGroup<G>::groups) {
+    for (uint32_t row = blockIdx.x * ForwardGroup<G>::groups + threadIdx.x / G; row < sh.rows; row += gridDim.x * ForwardGroup<G>::groups) {
         const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
         const float first = x[at];
         float v[U][4];
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
                 const double d = static_cast<double>(v[u][e]) - k;
                 s[0] += d; s[1] = fma(d, d, s[1]);
             }
-        row_fold<G, 2>(s, lds, set);
+        row_fold<G, ForwardGroup<G>::threads, 2>(s, lds, set);
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -221,11 +225,11 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_forward_rows_kernel(c
 // leaves one row [2, cols] of partial sums as floats, each rounded once (2^-24 of itself), which ln_fold_kernel adds in f64;
 // one that is alone (no `partial`) writes the weights' gradients themselves.
 template <int G, int U>
-__global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
+__global__ __launch_bounds__((BackwardGroup<G, U>::threads)) void ln_backward_rows_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
                                                                                 float* __restrict__ partial, float* __restrict__ grad_gamma, float* __restrict__ grad_beta,
                                                                                 Shape2 sh, double eps) {
-    constexpr int threads = RowGroup<G>::threads, groups = RowGroup<G>::groups;
-    __shared__ double lds[G > 64 ? 2 * 4 * RowGroup<G>::waves : threads * 4];
+    constexpr int threads = BackwardGroup<G, U>::threads, groups = BackwardGroup<G, U>::groups;
+    __shared__ double lds[groups > 1 ? threads * 4 : 2 * 4 * threads / 64];    // (rows' sums, then the columns' sums)
     const uint32_t lane = threadIdx.x % G;
     uint32_t set = 0;
     float ga[U][4];
@@ -236,7 +240,11 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
         for (int e = 0; e < 4; e++) { ga[u][e] = 1.0f; sg[u][e] = 0.0; sb[u][e] = 0.0; }
         if (gamma) load4<false>(gamma, (u * G + lane) * 4, sh.cols, 1.0f, ga[u]);
     }
-    for (uint32_t row = blockIdx.x * groups + threadIdx.x / G; row < sh.rows; row += gridDim.x * groups) {
+    // (rows that several waves share meet at barriers: a workgroup's last rows may be none, which read the last one again)
+    constexpr bool meet = G > 64 && groups > 1;
+    for (uint32_t row0 = blockIdx.x * groups + (meet ? 0 : threadIdx.x / G); row0 < sh.rows; row0 += gridDim.x * groups) {
+        const uint32_t row = meet ? min(row0 + threadIdx.x / G, sh.rows - 1) : row0;
+        const bool none = meet && row0 + threadIdx.x / G >= sh.rows;
         const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
         const float first = x[at];
         float v[U][4], g[U][4];
@@ -256,7 +264,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
                 s[0] += d; s[1] = fma(d, d, s[1]); s[2] += w; s[3] = fma(w, d, s[3]);
                 KTH_FEW_AT_A_TIME(e);
             }
-        row_fold<G, 4>(s, lds, set);
+        row_fold<G, threads, 4>(s, lds, set);
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -264,6 +272,7 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
         const double inv = sh.inv_cols, delta = s[0] * inv, mean = k + delta;
         const double rstd = row_rstd_fast(row_variance(s[0], s[1], inv), eps);
         const double w_mean = s[2] * inv, dot = (s[3] - delta * s[2]) * rstd * rstd * inv;
+        if (none) break;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float r[4];
@@ -286,21 +295,23 @@ __global__ __launch_bounds__(RowGroup<G>::threads) void ln_backward_rows_kernel(
 #pragma unroll
         for (int which = 0; which < 2; which++) {
             double (&t)[4] = which == 0 ? sg[u] : sb[u];
-            if constexpr (groups > 1) {                        // the workgroup's rows side by side, lane by lane
+            float* to = partial ? mine + which * sh.cols : which == 0 ? grad_gamma : grad_beta;
+            if constexpr (groups > 1) {                        // the workgroup's rows side by side, its threads on the columns
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < 4; e++) lds[e * threads + threadIdx.x] = t[e];
                 __syncthreads();
-                if (threadIdx.x < G)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        for (int r = 1; r < groups; r++) t[e] += lds[e * threads + r * G + threadIdx.x];
-            }
-            if (threadIdx.x < G) {
+                for (uint32_t e = threadIdx.x / G; e < 4; e += groups) {
+                    const uint32_t c = (u * G + lane) * 4 + e;
+                    if (!to || c >= sh.cols) continue;
+                    double sum = lds[e * threads + lane];
+                    for (int r = 1; r < groups; r++) sum += lds[e * threads + r * G + lane];
+                    to[c] = static_cast<float>(sum);
+                }
+            } else {
                 float f[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) f[e] = static_cast<float>(t[e]);
-                float* to = partial ? mine + which * sh.cols : which == 0 ? grad_gamma : grad_beta;
                 if (to) store4(to, (u * G + lane) * 4, sh.cols, f);
             }
         }
@@ -562,7 +573,7 @@ struct ForwardRows {
 };
 template <int G, int U>
 ForwardRows forward_rows_of(const Shape2& sh, uint32_t per_unit) {
-    return ForwardRows{ln_forward_rows_kernel<G, U>, RowGroup<G>::threads, grid_for(sh, RowGroup<G>::groups, per_unit)};
+    return ForwardRows{ln_forward_rows_kernel<G, U>, ForwardGroup<G>::threads, grid_for(sh, ForwardGroup<G>::groups, per_unit)};
 }
 ForwardRows forward_rows_kernel(const Shape2& sh) {
     const uint32_t c = sh.cols;
@@ -579,16 +590,17 @@ struct BackwardRows {
 };
 template <int G, int U>
 BackwardRows backward_rows_of(const Shape2& sh, uint32_t per_unit) {
-    return BackwardRows{ln_backward_rows_kernel<G, U>, RowGroup<G>::threads, grid_for(sh, RowGroup<G>::groups, per_unit)};
+    return BackwardRows{ln_backward_rows_kernel<G, U>, BackwardGroup<G, U>::threads, grid_for(sh, BackwardGroup<G, U>::groups, per_unit)};
 }
 BackwardRows backward_rows_kernel(const Shape2& sh) {
     const uint32_t c = sh.cols;
-    // Four float4s a lane are the fastest where there are rows enough for the chip ([65536,1024] 147 us against 217 with
-    // one); with few rows a row is spread over a workgroup.
-    if (c > 512 && c <= 1024 && sh.rows <= 4 * device_units()) return backward_rows_of<256, 1>(sh, 4);
-    return c <= 16 ? backward_rows_of<4, 1>(sh, 6) : c <= 64 ? backward_rows_of<16, 1>(sh, 6) : c <= 128 ? backward_rows_of<16, 2>(sh, 4)
-         : c <= 256 ? backward_rows_of<64, 1>(sh, 6) : c <= 512 ? backward_rows_of<64, 2>(sh, 4) : c <= 768 ? backward_rows_of<64, 3>(sh, 3)
-         : c <= 1024 ? backward_rows_of<64, 4>(sh, 2) : c <= 2048 ? backward_rows_of<128, 4>(sh, 4) : c <= 4096 ? backward_rows_of<256, 4>(sh, 2)
+    // Four float4s a lane are the fastest where there are rows enough for the chip ([65536,1024] 150 us against 217 with
+    // one, [1000,1024] 11.0 against 13.6); fewer rows are spread over four waves each ([500,1024] 9.3 us against 10.0,
+    // [100,1024] 7.4 against 9.7).
+    if (c > 512 && c <= 1024 && sh.rows <= 2 * device_units()) return backward_rows_of<256, 1>(sh, 2);
+    return c <= 16 ? backward_rows_of<4, 1>(sh, 3) : c <= 64 ? backward_rows_of<16, 1>(sh, 3) : c <= 128 ? backward_rows_of<16, 2>(sh, 2)
+         : c <= 256 ? backward_rows_of<64, 1>(sh, 3) : c <= 512 ? backward_rows_of<64, 2>(sh, 2) : c <= 768 ? backward_rows_of<64, 3>(sh, 1)
+         : c <= 1024 ? backward_rows_of<64, 4>(sh, 1) : c <= 2048 ? backward_rows_of<128, 4>(sh, 1) : c <= 4096 ? backward_rows_of<256, 4>(sh, 2)
          : backward_rows_of<1024, 2>(sh, 1);
 }
 
