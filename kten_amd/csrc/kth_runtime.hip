@@ -180,19 +180,23 @@ Store* lookup_index(uint64_t handle, const char* what) {
 }
 
 int resolve_operands(const char* what, Operand* ops, int count, std::initializer_list<std::pair<int, int>> allowed, int size_code) {
-    char label[96];
+    State& s = state();
     for (int i = 0; i < count; i++) {
         Operand& o = ops[i];
         if (o.handle == 0) continue;
-        snprintf(label, sizeof label, "%s(%s)", what, o.name);
-        o.store = lookup_unsettled(o.handle, label, true, true);       // (nothing is done to it yet)
-        if (!o.store) return KTH_E_HANDLE;
-        if (o.store->n_floats < o.n)
-            return fail(size_code, "%s holds %llu values, %llu are needed", label, (unsigned long long)o.store->n_floats, (unsigned long long)o.n);
+        const uint32_t low = static_cast<uint32_t>(o.handle & 0xffffffffu);
+        Store* st = low != 0 && low <= s.table.size() ? &s.table[low - 1] : nullptr;
+        if (!st || st->refs == 0 || st->generation != static_cast<uint32_t>(o.handle >> 32) || st->n_floats < o.n) {
+            char label[96];                                            // (made for a refusal only: it costs as much as the rest)
+            snprintf(label, sizeof label, "%s(%s)", what, o.name);
+            if (!lookup_unsettled(o.handle, label, true, true)) return KTH_E_HANDLE;
+            return fail(size_code, "%s holds %llu values, %llu are needed", label, (unsigned long long)st->n_floats, (unsigned long long)o.n);
+        }
+        o.store = st;
     }
     for (int i = 0; i < count; i++)
-        for (int j = 0; j < count; j++) {
-            if (i == j || !ops[i].result || !ops[i].store || ops[i].store != ops[j].store) continue;
+        for (int j = 0; ops[i].result && ops[i].store && j < count; j++) {
+            if (i == j || ops[i].store != ops[j].store) continue;
             bool fine = false;
             for (const std::pair<int, int>& p : allowed) fine = fine || (p.first == i && p.second == j);
             if (!fine) return fail(KTH_E_ARGUMENT, "%s: %s and %s are the same store", what, ops[i].name, ops[j].name);
