@@ -214,7 +214,7 @@ struct TilePlan {
 
 struct Pair { double A, H; };
 
-// Keeps the instructions of few steps at a time in flight, for the same reason.
+// Keeps the instructions of few steps at a time in flight: the f64 values of all of them would not fit a lane's registers.
 #define KTH_STEPS_APART(k) do { if ((k) % 4 == 3) __builtin_amdgcn_sched_barrier(0); } while (0)
 
 // Where a workgroup and its waves stand.

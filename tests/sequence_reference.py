@@ -1,7 +1,7 @@
 """Layer norm, dropout and the gated linear recurrence from their definitions in float64 (numpy), each with a bound on what
 a correct float kernel may differ by: u = 2^-24 is half a step of a float, w = 2^-53 that of a double.
 
-`SequenceOracleOperations` puts them behind the CPU checker's raw tensors, so that the autograd layer runs on the CPU."""
+`SequenceOracleOperations` puts them behind the oracle's raw tensors, so that the autograd layer runs on the CPU."""
 import numpy as np
 
 from kten_amd.host_mirror import shape_functions as sf
@@ -197,7 +197,7 @@ def recurrence_grad_bounds(gate, x, initial, h, go, grad_final, sigmoid):
     return np.abs(before) * (off + 2 * U * size) + 1e-44, off + 2 * U * size + 1e-44, b_initial
 
 
-# ---------------------------------------------------------------- behind the CPU checker's raw tensors
+# ---------------------------------------------------------------- behind the oracle's raw tensors
 
 def _view(raw, *shape):
     return None if raw is None else raw.toArray().reshape(*shape)
