@@ -317,7 +317,97 @@ __global__ __launch_bounds__((BackwardGroup<G, U>::threads)) void ln_backward_ro
         }
 }
 
-// ---------------------------------------------------------------- longer rows, in segments
+// ---------------------------------------------------------------- longer rows, in LDS and registers
+
+// A workgroup of 1024 threads holds a row: R float4s a lane in registers, the columns after them in LDS, where a lane reads
+// back only what it wrote (the barrier of the row's sums is the only one). The weights are read again for every row, from
+// the cache.
+constexpr uint32_t kLongThreads = 1024, kLdsRowFloats = 36864;
+template <int R>
+__global__ __launch_bounds__(kLongThreads) void ln_forward_long_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* out,
+                                                                       float* __restrict__ out_mean, float* __restrict__ out_std, Shape2 sh, double eps) {
+    extern __shared__ float4 held[];
+    __shared__ double lds[2 * 2 * kLongThreads / 64];
+    constexpr uint32_t after = R * kLongThreads * 4;         // the first column that lies in LDS
+    constexpr uint32_t kInFlight = 4;
+    const uint32_t many = (sh.cols - after + 3) / 4;         // float4s in LDS
+    uint32_t set = 0;
+    for (uint32_t row = blockIdx.x; row < sh.rows; row += gridDim.x) {
+        const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
+        const float first = x[at];
+        const double k = static_cast<double>(first);
+        double s[2] = {};
+        v4f_any v[R > 0 ? R : 1];                            // (columns that every such row has)
+#pragma unroll
+        for (int u = 0; u < R; u++) v[u] = *reinterpret_cast<const v4f_any*>(x + at + (u * kLongThreads + threadIdx.x) * 4);
+        for (uint32_t i0 = threadIdx.x; i0 < many; i0 += kInFlight * kLongThreads) {
+            float t[kInFlight][4];
+#pragma unroll
+            for (uint32_t j = 0; j < kInFlight; j++) {
+                const uint32_t i = i0 + j * kLongThreads;
+                if (i < many) load4<false>(x + at, after + i * 4, sh.cols, first, t[j]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kInFlight; j++) {
+                const uint32_t i = i0 + j * kLongThreads;
+                if (i < many) {
+                    held[i] = float4{t[j][0], t[j][1], t[j][2], t[j][3]};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const double d = static_cast<double>(t[j][e]) - k;
+                        s[0] += d; s[1] = fma(d, d, s[1]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < R; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double d = static_cast<double>(v[u][e]) - k;
+                s[0] += d; s[1] = fma(d, d, s[1]);
+                KTH_FEW_AT_A_TIME(e);
+            }
+        row_fold<kLongThreads, kLongThreads, 2>(s, lds, set);
+#pragma unroll
+        for (int u = 0; u < R; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) { float keep = v[u][e]; forget(keep); v[u][e] = keep; }
+        const double mean = k + s[0] * sh.inv_cols;
+        const double rstd = row_rstd_fast(row_variance(s[0], s[1], sh.inv_cols), eps);
+        auto apply = [&](const float (&t)[4], uint32_t c) {
+            float ga[4] = {1.0f, 1.0f, 1.0f, 1.0f}, be[4] = {}, y[4];
+            if (gamma) load4<false>(gamma, c, sh.cols, 1.0f, ga);
+            if (beta) load4<false>(beta, c, sh.cols, 0.0f, be);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = ln_forward(t[e], mean, rstd, ga[e], be[e]);
+            store4(out + at, c, sh.cols, y);
+        };
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+            const uint32_t c = (u * kLongThreads + threadIdx.x) * 4;
+            v4f_any ga{1.0f, 1.0f, 1.0f, 1.0f}, be{}, y;
+            if (gamma) ga = *reinterpret_cast<const v4f_any*>(gamma + c);
+            if (beta) be = *reinterpret_cast<const v4f_any*>(beta + c);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = ln_forward(v[u][e], mean, rstd, ga[e], be[e]);
+            *reinterpret_cast<v4f_any*>(out + at + c) = y;
+            if (u % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll 2
+        for (uint32_t i = threadIdx.x; i < many; i += kLongThreads) {
+            const float4 h = held[i];
+            const float t[4] = {h.x, h.y, h.z, h.w};
+            apply(t, after + i * 4);
+        }
+        if (threadIdx.x == 0) {
+            if (out_mean) out_mean[row] = static_cast<float>(mean);
+            if (out_std) out_std[row] = static_cast<float>(rstd);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the same in segments
 
 struct SegPlan {
     Shape2   sh;
@@ -554,9 +644,14 @@ SegPlan plan_segments(const Shape2& sh) {
     return pl;
 }
 
-// The widest rows that stay in registers. (With 8 float4s a lane, up to 32768 columns, the forward kernel spills: 82 us for
-// [1000,30000], as much as in segments.)
+// The widest rows that stay in registers. (With 8 float4s a lane the forward kernel spills.)
 constexpr uint32_t kForwardRowCols = 16384, kBackwardRowCols = 8192;
+
+// Rows that ln_forward_long_kernel takes: those that LDS holds, and longer ones where there are rows enough (segments / a
+// workgroup a row, us: [1,20000] 8.9 / 5.7, [64,36000] 11.9 / 11.1, [1000,30000] 81 / 64; [32,65536] 10.9 / 15.8, [100,65536] 18.5 / 18.0,
+// [1000,65536] 188 / 123).
+constexpr int kLongRegisters = 7;
+constexpr uint32_t kLongRowCols = kLdsRowFloats + kLongRegisters * kLongThreads * 4, kLongRows = 96;
 
 uint32_t grid_for(const Shape2& sh, uint32_t groups, uint32_t per_unit) {
     return std::min((sh.rows - 1) / groups + 1, device_units() * per_unit);       // (fewer than 2^32 threads in all)
@@ -584,6 +679,18 @@ ForwardRows forward_rows_kernel(const Shape2& sh) {
          : c <= 8192 ? forward_rows_of<512, 4>(sh, 2) : forward_rows_of<1024, 4>(sh, 1);
 }
 
+// A workgroup may use 64 KiB of dynamic LDS unless the kernel is granted more.
+bool long_rows_allowed() {
+    static const bool allowed = [] {
+        bool ok = true;
+        for (const void* f : {reinterpret_cast<const void*>(&ln_forward_long_kernel<0>), reinterpret_cast<const void*>(&ln_forward_long_kernel<kLongRegisters>)})
+            ok = ok && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsRowFloats * 4) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
+        return ok;
+    }();
+    return allowed;
+}
+
 struct BackwardRows {
     void (*kernel)(const float*, const float*, const float*, float*, float*, float*, float*, Shape2, double);
     uint32_t threads, grid;
@@ -606,10 +713,10 @@ BackwardRows backward_rows_kernel(const Shape2& sh) {
 
 void launch_fold(const float* partial, uint32_t cols, uint32_t ranges, float* grad_gamma, float* grad_beta) {
     LaunchScope scope("ln_fold_kernel", "", static_cast<uint64_t>(ranges) * 2 * cols * sizeof(float));
-    const uint32_t lanes = ranges <= 16 ? 4 : 64, per_block = kFoldBlock / lanes;
+    const uint32_t lanes = ranges <= 16 ? 4 : ranges <= 128 ? 16 : 64, per_block = kFoldBlock / lanes;
     const dim3 grid(std::min((cols - 1) / per_block + 1, kMaxFoldGrid), 2);
-    if (lanes == 4) hipLaunchKernelGGL((ln_fold_kernel<4>), grid, dim3(kFoldBlock), 0, state().stream, partial, cols, ranges, grad_gamma, grad_beta);
-    else            hipLaunchKernelGGL((ln_fold_kernel<64>), grid, dim3(kFoldBlock), 0, state().stream, partial, cols, ranges, grad_gamma, grad_beta);
+    auto* kernel = lanes == 4 ? ln_fold_kernel<4> : lanes == 16 ? ln_fold_kernel<16> : ln_fold_kernel<64>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kFoldBlock), 0, state().stream, partial, cols, ranges, grad_gamma, grad_beta);
 }
 
 uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
@@ -636,6 +743,17 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
         LaunchScope scope("ln_forward_rows_kernel", "", n * 8);
         const ForwardRows k = forward_rows_kernel(sh);
         hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pga, pbe, pout, pmean, pstd, sh, static_cast<double>(epsilon));
+        KTH_LAUNCH_CHECK("layer_norm_forward");
+        return KTH_OK;
+    }
+    if (sh.cols <= (sh.rows >= kLongRows ? kLongRowCols : kLdsRowFloats) && long_rows_allowed()) {
+        LaunchScope scope("ln_forward_long_kernel", "", n * 8);
+        const bool lds_alone = sh.cols <= kLdsRowFloats;
+        const uint32_t held = lds_alone ? sh.cols : sh.cols - kLongRegisters * kLongThreads * 4;
+        const uint32_t lds = (held + 3) / 4 * 16;
+        const dim3 grid(std::min(sh.rows, device_units() * (lds <= 72 * 1024 ? 2u : 1u)));
+        auto* kernel = lds_alone ? ln_forward_long_kernel<0> : ln_forward_long_kernel<kLongRegisters>;
+        hipLaunchKernelGGL(kernel, grid, dim3(kLongThreads), lds, state().stream, px, pga, pbe, pout, pmean, pstd, sh, static_cast<double>(epsilon));
         KTH_LAUNCH_CHECK("layer_norm_forward");
         return KTH_OK;
     }

@@ -61,6 +61,22 @@ def test_many_rows(shape, gc):
     check_backward(gc, x, gamma, go)
 
 
+@pytest.mark.parametrize("shape", [(64, 16385), (300, 20003), (65, 36864), (64, 36865), (63, 40000), (520, 17000), (64, 65536), (70, 65533), (64, 65537)],
+                         ids=lambda s: f"{s[0]}x{s[1]}")
+def test_long_rows(shape, gc):
+    x, go = data(1, *shape) + np.float32(0.5), data(2, *shape)
+    gamma, beta = data(3, shape[1]), data(4, shape[1])
+    check_forward(gc, x, gamma, beta)
+    check_forward(gc, x, None, None)
+    check_backward(gc, x, gamma, go)
+    # the result over its input, with the statistics left out
+    raw = [gc.createRaw(list(a.shape), a) for a in (x, gamma, beta)]
+    want = gc.layerNorm(1, EPS).calculateOutput(*raw)[0].toArray()
+    abi.check(gc.lib.kth_layer_norm_forward(raw[0].storeReference, abi.shape_array(shape), 2, 1, EPS, raw[1].storeReference, raw[2].storeReference,
+                                            raw[0].storeReference, 0, 0))
+    assert_bits_equal(raw[0].toArray(), want, "in place")
+
+
 @pytest.mark.parametrize("shape", [(37, 60), (37, 300), (20, 1500), (10, 5000), (6, 20000)], ids=lambda s: f"{s[0]}x{s[1]}")
 def test_absent_operands_and_results(shape, gc):
     x, go, gamma, beta = data(1, *shape), data(2, *shape), data(3, shape[1]), data(4, shape[1])
