@@ -169,6 +169,7 @@ __device__ __forceinline__ void store4(float* p, uint32_t c, uint32_t cols, cons
     }
 }
 
+// Bound by memory: [16384,4096] 94.7 us, 5.7 TB/s; [8191,1021] 13.8 us, 4.9 TB/s, a round of workgroups and its start and end.
 template <int G, int U>
 __global__ __launch_bounds__(ForwardGroup<G>::threads) void ln_forward_rows_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta,
                                                                                float* out, float* __restrict__ out_mean, float* __restrict__ out_std,
@@ -223,7 +224,8 @@ __global__ __launch_bounds__(ForwardGroup<G>::threads) void ln_forward_rows_kern
 
 // The input gradient of each row, and down the workgroup's rows the weights' gradients, in f64 registers; a workgroup
 // leaves one row [2, cols] of partial sums as floats, each rounded once (2^-24 of itself), which ln_fold_kernel adds in f64;
-// one that is alone (no `partial`) writes the weights' gradients themselves.
+// one that is alone (no `partial`) writes the weights' gradients themselves. Bound by memory where there are rows enough:
+// [16384,4096] 147.6 us with the fold, 5.5 TB/s; [8192,768] 20.6 us, of which the fold's launch takes 4.
 template <int G, int U>
 __global__ __launch_bounds__((BackwardGroup<G, U>::threads)) void ln_backward_rows_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
                                                                                 float* __restrict__ partial, float* __restrict__ grad_gamma, float* __restrict__ grad_beta,
@@ -321,7 +323,7 @@ __global__ __launch_bounds__((BackwardGroup<G, U>::threads)) void ln_backward_ro
 
 // A workgroup of 1024 threads holds a row: R float4s a lane in registers, the columns after them in LDS, where a lane reads
 // back only what it wrote (the barrier of the row's sums is the only one). The weights are read again for every row, from
-// the cache.
+// the cache. [1000,30000] 64 us, 3.7 TB/s: a compute unit has one row at a time, and reads nothing while it writes.
 constexpr uint32_t kLongThreads = 1024, kLdsRowFloats = 36864;
 template <int R>
 __global__ __launch_bounds__(kLongThreads) void ln_forward_long_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* out,
@@ -459,6 +461,36 @@ __global__ __launch_bounds__(kBlock) void ln_sums_kernel(const float* __restrict
         for (int i = 0; i < NS; i++) partial[static_cast<uint64_t>(b) * NS + i] = s[i];
 }
 
+// The statistics of the backward pass where a workgroup sums a whole row: in segments / whole, us for the pass: [1,10000] 9.0 /
+// 7.2, [100,10000] 21.8 / 19.0, [500,9000] 29.4 / 25.9, [2000,10000] 91 / 86, [1000,65536] 277 / 269; but [64,65536] 27 / 29 and
+// [8,1000000] 66 / 239, a few long rows, which leave most of the chip idle.
+__global__ __launch_bounds__(kLongThreads) void ln_row_sums_kernel(const float* __restrict__ x, const float* __restrict__ go, const float* __restrict__ gamma,
+                                                                   RowBackward* __restrict__ rows, Shape2 sh, double eps) {
+    __shared__ double lds[2 * 4 * kLongThreads / 64];
+    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * sh.cols;
+    const float first = x[at];
+    const double k = static_cast<double>(first);
+    double s[4] = {};
+    for (uint32_t c = threadIdx.x * 4; c < sh.cols; c += kLongThreads * 4) {
+        float v[4], g[4], ga[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        load4<false>(x + at, c, sh.cols, first, v);                    // (behind the last column terms of zero)
+        load4<false>(go + at, c, sh.cols, 0.0f, g);
+        if (gamma) load4<false>(gamma, c, sh.cols, 1.0f, ga);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double d = static_cast<double>(v[e]) - k;
+            const double w = static_cast<double>(g[e]) * static_cast<double>(ga[e]);
+            s[0] += d; s[1] = fma(d, d, s[1]); s[2] += w; s[3] = fma(w, d, s[3]);
+        }
+    }
+    uint32_t set = 0;
+    row_fold<kLongThreads, kLongThreads, 4>(s, lds, set);
+    if (threadIdx.x != 0) return;
+    const double inv = sh.inv_cols, delta = s[0] * inv;
+    const double rstd = row_rstd_fast(row_variance(s[0], s[1], inv), eps);
+    rows[blockIdx.x] = RowBackward{k + delta, rstd, s[2] * inv, (s[3] - delta * s[2]) * rstd * rstd * inv};
+}
+
 // One wave per row folds its segments (lane l takes l, l + 64, ...; then the lanes by xor-shuffles).
 template <bool BACKWARD>
 __global__ __launch_bounds__(kBlock) void ln_rows_kernel(const float* __restrict__ x, const double* __restrict__ partial, SegPlan pl, double eps,
@@ -521,7 +553,7 @@ struct ColPlan {
     FastDiv  col_div;
 };
 
-// A thread owns four columns of one range of rows: it writes the input gradient of each row and sums the weights'
+// ([2000,10000] 41 us, 5.8 TB/s.) A thread owns four columns of one range of rows: it writes the input gradient of each row and sums the weights'
 // gradients down the range. The partials are floats: each is a f64 sum rounded once (2^-24 of itself), folded in f64.
 __global__ __launch_bounds__(kBlock) void ln_cols_kernel(const float* __restrict__ x, const float* go, const float* __restrict__ gamma, float* grad_in,
                                                          const RowBackward* __restrict__ rows, float* __restrict__ partial, float* __restrict__ grad_gamma,
@@ -651,6 +683,8 @@ constexpr uint32_t kForwardRowCols = 16384, kBackwardRowCols = 8192;
 // workgroup a row, us: [1,20000] 8.9 / 5.7, [64,36000] 11.9 / 11.1, [1000,30000] 81 / 64; [32,65536] 10.9 / 15.8, [100,65536] 18.5 / 18.0,
 // [1000,65536] 188 / 123).
 constexpr int kLongRegisters = 7;
+// Rows that ln_row_sums_kernel takes: up to so many columns, or longer ones where every compute unit has two.
+constexpr uint32_t kWholeRowCols = 32768;
 constexpr uint32_t kLongRowCols = kLdsRowFloats + kLongRegisters * kLongThreads * 4, kLongRows = 96;
 
 uint32_t grid_for(const Shape2& sh, uint32_t groups, uint32_t per_unit) {
@@ -829,7 +863,8 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     const bool weights = (pgg || pgb) && cp.ranges > 1;
     const uint64_t blocks = static_cast<uint64_t>(sh.rows) * pl.segments;
     const uint64_t rows_bytes = align256(static_cast<uint64_t>(sh.rows) * sizeof(RowBackward));
-    const uint64_t sums_bytes = align256(blocks * 4 * sizeof(double));
+    const bool whole_rows = sh.cols <= kWholeRowCols || sh.rows >= 2 * device_units();
+    const uint64_t sums_bytes = whole_rows ? 0 : align256(blocks * 4 * sizeof(double));
     const uint64_t cols_bytes = weights ? static_cast<uint64_t>(cp.ranges) * 2 * sh.cols * sizeof(float) : 0;
     const uint64_t ws_bytes = rows_bytes + sums_bytes + cols_bytes;
     uint64_t cap;
@@ -839,14 +874,19 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     double* sums = reinterpret_cast<double*>(ws + rows_bytes);
     float* partial = weights ? reinterpret_cast<float*>(ws + rows_bytes + sums_bytes) : nullptr;
     hipStream_t stream = state().stream;
-    {
-        LaunchScope scope("ln_sums_kernel", "backward", n * 8);
-        hipLaunchKernelGGL((ln_sums_kernel<true>), dim3(pl.blocks), dim3(kBlock), 0, stream, px, pgo, pga, sums, pl);
-    }
-    {
-        LaunchScope scope("ln_rows_kernel", "backward", blocks * 32);
-        hipLaunchKernelGGL((ln_rows_kernel<true>), dim3((sh.rows - 1) / 4 + 1), dim3(kBlock), 0, stream, px, sums, pl, static_cast<double>(epsilon),
-                           nullptr, rows, nullptr, nullptr);
+    if (whole_rows) {
+        LaunchScope scope("ln_row_sums_kernel", "", n * 8);
+        hipLaunchKernelGGL(ln_row_sums_kernel, dim3(sh.rows), dim3(kLongThreads), 0, stream, px, pgo, pga, rows, sh, static_cast<double>(epsilon));
+    } else {
+        {
+            LaunchScope scope("ln_sums_kernel", "backward", n * 8);
+            hipLaunchKernelGGL((ln_sums_kernel<true>), dim3(pl.blocks), dim3(kBlock), 0, stream, px, pgo, pga, sums, pl);
+        }
+        {
+            LaunchScope scope("ln_rows_kernel", "backward", blocks * 32);
+            hipLaunchKernelGGL((ln_rows_kernel<true>), dim3((sh.rows - 1) / 4 + 1), dim3(kBlock), 0, stream, px, sums, pl, static_cast<double>(epsilon),
+                               nullptr, rows, nullptr, nullptr);
+        }
     }
     {
         LaunchScope scope("ln_cols_kernel", "", n * (pgi ? 12 : 8) + cols_bytes);

@@ -64,7 +64,8 @@ __device__ __forceinline__ float sigmoid_b(float v) {
     return __int_as_float((__float_as_int(v) >> 31) & 0x3f800000) + v;   // 1 or 0
 }
 
-// A thread per channel walks its steps.
+// A thread per channel walks its steps: for one step a launch and little else ([64,1,1024] 2.7 us), for many channels bound by
+// memory ([100000,20,24] forward 127 us, 4.5 TB/s).
 template <bool SIGMOID>
 __global__ __launch_bounds__(kBlock) void recurrence_forward_kernel(const float* __restrict__ gate, const float* __restrict__ in, const float* initial,
                                                                     float* __restrict__ out, float* final_state, ScanShape sh) {
@@ -149,6 +150,11 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 // A published value is one 64-bit word that carries its own sign of life, a double whose last kTagBits bits hold the
 // launch's number: no fence, no flag, no clearing between launches (the words are cleared when the number starts again).
 // What the doubles lose is 2^-41 of themselves a tile.
+//
+// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 88 (4.6), backward 143 (4.7), [5,1999,1001] sigmoid
+// backward 69 (3.5; odd rows share cache lines with their neighbours). What bounds it is a tile's life, loads, the wait for
+// the state, stores, with two tiles in a compute unit's registers: the vector ALU is 40 % busy, and without the hand-over (its results
+// would be wrong) the same four take 46, 79, 122 and 68. Longer runs of steps spill, shorter ones have more tiles to hand over.
 constexpr int kTagBits = 12;
 constexpr uint32_t kTags = (1u << kTagBits) - 1;     // tag 0: never published
 constexpr uint32_t kSuper = 16;
@@ -428,7 +434,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
 // takes a stretch of up to 4096 floats as memory has them, through LDS, and a thread kSub steps of one channel: thread
 // (row, j, channel), j counting the kSub-step pieces of a row. Rows that fit are taken several at a time; longer ones are
 // cut into tiles that hand a state on as above. A piece's place in LDS is padded by one float, so that the threads of a
-// wave, a piece apart, do not meet in a bank.
+// wave, a piece apart, do not meet in a bank. [100000,64,1] 38 us forward (2.0 TB/s) and 87 backward, bound by the LDS and the
+// barriers of the scan over the pieces.
 constexpr uint32_t kNarrowThreads = 256, kSub = 16, kNarrowInner = 32;     // (inner is below kNarrowInner)
 constexpr uint32_t kNarrowFloats = kNarrowThreads * (kSub + 1);
 

@@ -61,7 +61,7 @@ def test_many_rows(shape, gc):
     check_backward(gc, x, gamma, go)
 
 
-@pytest.mark.parametrize("shape", [(64, 16385), (300, 20003), (65, 36864), (64, 36865), (63, 40000), (520, 17000), (64, 65536), (70, 65533), (64, 65537)],
+@pytest.mark.parametrize("shape", [(64, 16385), (300, 20003), (65, 36864), (64, 36865), (63, 40000), (520, 17000), (64, 65536), (100, 65533), (64, 65537), (515, 33001)],
                          ids=lambda s: f"{s[0]}x{s[1]}")
 def test_long_rows(shape, gc):
     x, go = data(1, *shape) + np.float32(0.5), data(2, *shape)
