@@ -716,6 +716,7 @@ ForwardRows forward_rows_kernel(const Shape2& sh) {
 // A workgroup may use 64 KiB of dynamic LDS unless the kernel is granted more.
 bool long_rows_allowed() {
     static const bool allowed = [] {
+        const OnDevice here;
         bool ok = true;
         for (const void* f : {reinterpret_cast<const void*>(&ln_forward_long_kernel<0>), reinterpret_cast<const void*>(&ln_forward_long_kernel<kLongRegisters>)})
             ok = ok && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsRowFloats * 4) == hipSuccess;
