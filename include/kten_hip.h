@@ -401,8 +401,10 @@ int kth_dropout(uint64_t in, uint64_t n, double p, uint64_t seed, uint64_t offse
 /* The gated linear recurrence along `axis`, each position of the other dims (a channel) on its own: out_t = h_t, h_{-1} =
  * initial (one float a channel, in the order of the other dims; 0: zeros); final_state receives the last step's state or
  * is 0. One step at a time (shape[axis] == 1, initial and final_state the same store, which is then updated in place) is
- * the form for single tokens. An infinite gate (KTH_GATE_GIVEN) leaves its channel infinite or NaN from its step on. Long
- * sequences are cut into tiles that wait for one another inside the launch; should such a wait be given up (after seconds,
+ * the form for single tokens. An infinite gate (KTH_GATE_GIVEN) leaves its channel infinite or NaN from its step on. Given
+ * gates may decay and grow as they like: a state that falls below the range of a double is 0 from there on and one that
+ * grows past it infinite or NaN, as step by step; one that falls by more than 2^1022 within a few hundred steps
+ * counts as 0 already. Long sequences are cut into tiles that wait for one another inside the launch; should such a wait be given up (after seconds,
  * on a device that stands still), the results behind it are NaN and the next kth_sync, kth_download or kth_read_scalar
  * returns KTH_E_DEVICE. */
 int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial,

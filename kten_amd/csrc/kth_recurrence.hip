@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 // launch's number: no fence, no flag, no clearing between launches (the words are cleared when the number starts again).
 // What the doubles lose is 2^-41 of themselves a tile.
 //
-// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 88 (4.6), backward 143 (4.7), [5,1999,1001] sigmoid
+// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 90 (4.5), backward 146 (4.6), [5,1999,1001] sigmoid
 // backward 69 (3.5; odd rows share cache lines with their neighbours). What bounds it is a tile's life, loads, the wait for
 // the state, stores, with two tiles in a compute unit's registers: the vector ALU is 40 % busy, and without the hand-over (its results
 // would be wrong) the same four take 46, 79, 122 and 68. Longer runs of steps spill, shorter ones have more tiles to hand over.
@@ -179,28 +179,64 @@ __device__ __forceinline__ double await(const uint64_t* word, uint32_t tag, int*
     return __longlong_as_double(static_cast<long long>(bits & ~static_cast<uint64_t>(kTags)));
 }
 
-// A state that is zero stays so, whatever the product of the gates (which may have overflowed).
-__device__ __forceinline__ double advance(double A, double H, double state) { return state == 0.0 ? H : fma(A, state, H); }
-
-// A product of gates none of which is zero does not become zero either (an infinite state stays infinite under any decay):
-// below the normal range it stays at that range's end, which moves no finite state that fp32 can hold.
+// The map K -> A K + H of a run of steps, A the product of its gates. A product of gates none of which is zero does not become
+// zero: below the normal range it is kLeast, of which an infinite state stays infinite. Where gates are given, and
+// may be above one, it stays kLeast whatever follows, and of a finite state it leaves nothing.
+struct Pair { double A, H; };
 constexpr double kLeast = 2.2250738585072014e-308;       // 2^-1022
-__device__ __forceinline__ double product(double later, double earlier) {
-    const double r = later * earlier;
-    return fabs(r) < kLeast && later != 0.0 && earlier != 0.0 ? copysign(kLeast, r) : r;
-}
-// The same for the steps of one run, whose gates are multiplied to A one by one. `least` is kept by an instruction a step and
-// without a branch (a look at the gates where A is that small makes the compiler keep twice the registers: 48 to 78 us for
-// [8,2048,1024]); it tells whether a gate was zero, which is -0 where gates are packed logits, the smallest of all integers.
+
+// The state after the run.
 template <bool SIGMOID>
-struct Least {
-    float abs = INFINITY;
-    int   bits = INT_MAX;
-    __device__ __forceinline__ void take(float v) {
-        if (SIGMOID) bits = min(bits, __float_as_int(v)); else abs = fminf(abs, fabsf(v));
+__device__ __forceinline__ double advance(const Pair& p, double state) {
+    if (SIGMOID) return state == 0.0 ? p.H : fma(p.A, state, p.H);
+    const bool lost = fabs(p.A) <= kLeast;
+    return fma(lost && fabs(state) < INFINITY ? 0.0 : p.A, state, p.H);
+}
+template <bool SIGMOID>
+__device__ __forceinline__ Pair after(const Pair& later, const Pair& earlier) {
+    double A = later.A * earlier.A;
+    const bool lost = SIGMOID ? fabs(A) < kLeast : fabs(A) < kLeast || fabs(later.A) <= kLeast || fabs(earlier.A) <= kLeast;
+    if (lost && later.A != 0.0 && earlier.A != 0.0 && (SIGMOID || fabs(A) < INFINITY)) A = copysign(kLeast, A);
+    return Pair{A, advance<SIGMOID>(later, earlier.H)};
+}
+// A run after which the state is known to be `end`, whatever came before; `state` is what did (an infinite one stays infinite or
+// becomes NaN).
+__device__ __forceinline__ Pair known(double state, double end) { return Pair{copysign(1.0, state) * copysign(kLeast, end), end}; }
+
+// The product of a run's gates, one by one. Whether a gate was zero is told by `abs` or `bits`, an instruction a step without
+// a branch (a look at the gates where A is that small makes the compiler keep twice the registers: 48 to 78 us for
+// [8,2048,1024]): -0 is a closed gate where gates are packed logits, the smallest of all integers.
+//
+// Runs are composed where they are tame: every product of sigmoids is, and one of given gates that is finite and (looked at every
+// fourth step) never more than 2^kRise above where it has been. Others, whose products may leave a double's range where the
+// states do not, or come back into it where the states are lost, are walked step by step once the state before them is known.
+// That costs a tile its independence: where every run rises by 2^18, [8,2048,1024] forward takes 52 us instead of 46, [1,65536,512]
+// 960 instead of 90, [1,66000,2] 864 instead of 14 (a thread a channel: 4419). Decays never rise, and gates of a normal
+// distribution or close to one hardly ever so far: they take the time of decays. A bound of 2^48 would still keep the products
+// of two tiles in range, but gates that halve and double a state by turns would then bring back what is lost on the way.
+constexpr int kRise = 16;
+template <bool SIGMOID>
+struct Product {
+    double A = 1.0;
+    float  abs = INFINITY;
+    int    bits = INT_MAX, low = 1023, rise = 0;         // exponents as a double's bits have them
+    __device__ __forceinline__ void look() {
+        const int now = __double2hiint(A) >> 20 & 0x7ff;
+        low = min(low, now);
+        rise = max(rise, now - low);
     }
-    __device__ __forceinline__ double keep(double A) const {
+    __device__ __forceinline__ void take(double a, float v, int k) {       // v: the gate as it is packed; k: the step's number in the run
+        A *= a;
+        if (SIGMOID) bits = min(bits, __float_as_int(v)); else abs = fminf(abs, fabsf(v));
+        if (!SIGMOID && k % 4 == 3) look();
+    }
+    __device__ __forceinline__ double gates() const {
         return fabs(A) < kLeast && (SIGMOID ? bits != INT_MIN : abs != 0.0f) ? copysign(kLeast, A) : A;
+    }
+    __device__ __forceinline__ bool tame() {
+        if (SIGMOID) return true;
+        look();
+        return rise <= kRise;                            // (an infinity or NaN is far above)
     }
 };
 
@@ -218,8 +254,6 @@ struct TilePlan {
     FastDiv  group_div, col_div;
 };
 
-struct Pair { double A, H; };
-
 // Keeps the instructions of few steps at a time in flight: the f64 values of all of them would not fit a lane's registers.
 #define KTH_STEPS_APART(k) do { if ((k) % 4 == 3) __builtin_amdgcn_sched_barrier(0); } while (0)
 
@@ -233,8 +267,9 @@ struct TilePlace {
     bool     valid;
 };
 
-__device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* lds_ticket) {
+__device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* lds_ticket, uint32_t* wild) {
     TilePlace w;
+    if (threadIdx.x == 0) *wild = 0;
     if (threadIdx.x == 0) *lds_ticket = pl.tiles > 1 ? atomicAdd(pl.tickets, 1u) : blockIdx.x;
     __syncthreads();
     const uint32_t ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
@@ -254,23 +289,25 @@ __device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* ld
     return w;
 }
 
-// The state before this wave's first step, from the pair (A, H) of its steps. `initial` is the state before the first
-// tile. lds: pairs of the waves, [tw][cw * 64], then of the tiles before, as many again.
-__device__ __forceinline__ double state_before(const TilePlan& pl, const TilePlace& w, double A, double H, double initial, Pair* lds) {
+// The state before this tile, from the pairs of its waves' steps and whether they are `tame`; `initial` is the state before
+// the first tile. lds: pairs of the waves, [tw][cw * 64], then of the tiles before, as many again; wild: 0 before the last
+// barrier. in_turn: a run of this tile is to be walked, so all are, one wave after another.
+template <bool SIGMOID>
+__device__ __forceinline__ double state_before_tile(const TilePlan& pl, const TilePlace& w, const Pair& mine, bool tame, double initial, Pair* lds, uint32_t* wild,
+                                                    bool& in_turn) {
     const uint32_t width = pl.cw * 64, at = w.cwi * 64 + w.lane;
     Pair* before = lds + pl.tw * width;
-    lds[w.twi * width + at] = Pair{A, H};
+    lds[w.twi * width + at] = mine;
+    if (!SIGMOID && !tame) *wild = 1;
     __syncthreads();
+    in_turn = !SIGMOID && __builtin_amdgcn_readfirstlane(*wild) != 0;
     double state = initial;
     const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
     if (pl.tiles > 1) {
-        if (w.twi == pl.tw - 1 && w.tile + 1 < pl.tiles && many + 1 < kSuper) {
+        if (w.twi == pl.tw - 1 && w.tile + 1 < pl.tiles && many + 1 < kSuper && !in_turn) {
             Pair total = lds[at];
-            for (uint32_t i = 1; i < pl.tw; i++) {
-                const Pair p = lds[i * width + at];
-                total = Pair{product(p.A, total.A), advance(p.A, p.H, total.H)};
-            }
-            if (w.tile == 0) total = Pair{0.0, advance(total.A, total.H, initial)};     // nobody else reads `initial`
+            for (uint32_t i = 1; i < pl.tw; i++) total = after<SIGMOID>(lds[i * width + at], total);
+            if (w.tile == 0) total = Pair{0.0, advance<SIGMOID>(total, initial)};     // nobody else reads `initial`
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
             publish(word, total.A, pl.tag);
             publish(word + 1, total.H, pl.tag);
@@ -283,21 +320,39 @@ __device__ __forceinline__ double state_before(const TilePlan& pl, const TilePla
             for (uint32_t i = from; i < to; i++) {
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + i) * pl.padded + w.slot) * 2;
                 const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
-                p = Pair{product(a, p.A), advance(a, h, p.H)};
+                p = after<SIGMOID>(Pair{a, h}, p);
             }
             before[w.twi * width + at] = p;
             state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag, pl.lost);
             __syncthreads();
-            for (uint32_t i = 0; i < pl.tw; i++) { const Pair q = before[i * width + at]; state = advance(q.A, q.H, state); }
-        }
-        if (w.twi == pl.tw - 1 && many + 1 == kSuper && w.tile + 1 < pl.tiles) {
-            double end = state;
-            for (uint32_t i = 0; i < pl.tw; i++) { const Pair q = lds[i * width + at]; end = advance(q.A, q.H, end); }
-            publish(pl.states + static_cast<uint64_t>(super) * pl.padded + w.slot, end, pl.tag);
+            for (uint32_t i = 0; i < pl.tw; i++) state = advance<SIGMOID>(before[i * width + at], state);
         }
     }
-    for (uint32_t i = 0; i < w.twi; i++) { const Pair q = lds[i * width + at]; state = advance(q.A, q.H, state); }
     return state;
+}
+// The state before this wave's first step from that before the tile, where the waves' pairs are composed.
+template <bool SIGMOID>
+__device__ __forceinline__ double state_before_wave(const TilePlan& pl, const TilePlace& w, double state, const Pair* lds) {
+    const uint32_t width = pl.cw * 64, at = w.cwi * 64 + w.lane;
+    if (w.twi == pl.tw - 1 && w.tile % kSuper + 1 == kSuper && w.tile + 1 < pl.tiles) {
+        double end = state;
+        for (uint32_t i = 0; i < pl.tw; i++) end = advance<SIGMOID>(lds[i * width + at], end);
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.tag);
+    }
+    for (uint32_t i = 0; i < w.twi; i++) state = advance<SIGMOID>(lds[i * width + at], state);
+    return state;
+}
+// What the last wave of a tile whose waves took turns hands on.
+__device__ __forceinline__ void hand_on_end(const TilePlan& pl, const TilePlace& w, double before_tile, double end) {
+    if (w.twi != pl.tw - 1 || w.tile + 1 >= pl.tiles) return;
+    if (w.tile % kSuper + 1 == kSuper) {
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.tag);
+    } else {
+        uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
+        const Pair total = known(before_tile, end);
+        publish(word, total.A, pl.tag);
+        publish(word + 1, total.H, pl.tag);
+    }
 }
 
 constexpr uint32_t kTileThreads = 512;
@@ -311,8 +366,8 @@ template <bool SIGMOID, bool LINES, int L>
 __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kernel(const float* __restrict__ gate, const float* __restrict__ in, const float* initial,
                                                                                    float* __restrict__ out, float* final_state, TilePlan pl) {
     extern __shared__ Pair lds[];
-    __shared__ uint32_t lds_ticket;
-    const TilePlace w = place_tile(pl, &lds_ticket);
+    __shared__ uint32_t lds_ticket, wild;
+    const TilePlace w = place_tile(pl, &lds_ticket, &wild);
     if (w.tile >= pl.tiles) return;
     const uint32_t t0 = (w.tile * pl.tw + w.twi) * L;
     const uint64_t row0 = w.base + static_cast<uint64_t>(t0) * pl.inner;
@@ -327,8 +382,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
     for (int k = 0; k < L; k++)                              // a step behind the last one leaves the state as it is
         if (t0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; u[k] = 0.0f; }
     const double start = w.tile == 0 && initial ? static_cast<double>(initial[w.first_state]) : 0.0;
-    double A = 1.0, H = 0.0;
-    Least<SIGMOID> least;
+    double H = 0.0;
+    Product<SIGMOID> product;
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (SIGMOID) {
@@ -337,13 +392,38 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
         }
         const double a = gate_a<SIGMOID>(v[k]);
         H = fma(a, H, static_cast<double>(u[k]));
-        A *= a;
-        least.take(v[k]);
+        product.take(a, v[k], k);
         KTH_STEPS_APART(k);
     }
 #pragma unroll
     for (int k = 0; k < L; k++) { forget(v[k]); forget(u[k]); }
-    double h = state_before(pl, w, least.keep(A), H, start, lds);
+    const Pair mine{product.gates(), H};
+    bool in_turn;
+    double h = state_before_tile<SIGMOID>(pl, w, mine, product.tame(), start, lds, &wild, in_turn);
+    if (in_turn) {
+        Pair* slot = lds + w.cwi * 64 + w.lane;              // wave i's of this channel: slot[i * width]; H: the state behind it
+        const uint32_t width = pl.cw * 64;
+        double end = h;
+        const double before_tile = h;
+        for (uint32_t i = 0; i < pl.tw; i++) {
+            if (i == w.twi) {
+                if (i > 0) h = slot[(i - 1) * width].H;
+                end = h;
+#pragma unroll
+                for (int k = 0; k < L; k++) { forget(v[k]); forget(u[k]); }
+#pragma unroll
+                for (int k = 0; k < L; k++) {
+                    end = fma(gate_a<SIGMOID>(v[k]), end, static_cast<double>(u[k]));
+                    KTH_STEPS_APART(k);
+                }
+                slot[i * width].H = end;
+            }
+            __syncthreads();
+        }
+        hand_on_end(pl, w, before_tile, end);
+    } else {
+        h = state_before_wave<SIGMOID>(pl, w, h, lds);
+    }
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (t0 + k < pl.steps) {
@@ -364,8 +444,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
                                                                                     float* __restrict__ grad_gate, float* __restrict__ grad_in,
                                                                                     float* __restrict__ grad_initial, TilePlan pl) {
     extern __shared__ Pair lds[];
-    __shared__ uint32_t lds_ticket;
-    const TilePlace w = place_tile(pl, &lds_ticket);
+    __shared__ uint32_t lds_ticket, wild;
+    const TilePlace w = place_tile(pl, &lds_ticket, &wild);
     if (w.tile >= pl.tiles) return;
     const uint32_t q0 = (w.tile * pl.tw + w.twi) * L;        // step t = steps - 1 - (q0 + k)
     const uint64_t last_row = w.base + static_cast<uint64_t>(pl.steps - 1) * pl.inner;
@@ -380,15 +460,14 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
     for (int k = 0; k < L; k++)
         if (q0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; g[k] = 0.0f; }
     const double start = w.tile == 0 && grad_final ? static_cast<double>(grad_final[w.first_state]) : 0.0;
-    double A = 1.0, H = 0.0;
-    Least<SIGMOID> least;
+    double H = 0.0;
+    Product<SIGMOID> product;
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (SIGMOID) v[k] = pack_gate<SIGMOID>(v[k]);
         const double a = gate_a<SIGMOID>(v[k]);
         H = a * (static_cast<double>(g[k]) + H);
-        A *= a;
-        least.take(v[k]);
+        product.take(a, v[k], k);
         KTH_STEPS_APART(k);
     }
 #pragma unroll
@@ -409,7 +488,33 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
             for (int k = 0; k < L; k++) if (q0 + k + 1 == pl.steps) before[k] = h0;
         }
     }
-    double K = state_before(pl, w, least.keep(A), H, start, lds);
+    const Pair mine{product.gates(), H};
+    bool in_turn;
+    double K = state_before_tile<SIGMOID>(pl, w, mine, product.tame(), start, lds, &wild, in_turn);
+    if (in_turn) {
+        Pair* slot = lds + w.cwi * 64 + w.lane;              // wave i's of this channel: slot[i * width]; H: the state behind it
+        const uint32_t width = pl.cw * 64;
+        double end = K;
+        const double before_tile = K;
+        for (uint32_t i = 0; i < pl.tw; i++) {
+            if (i == w.twi) {
+                if (i > 0) K = slot[(i - 1) * width].H;
+                end = K;
+#pragma unroll
+                for (int k = 0; k < L; k++) { forget(v[k]); forget(g[k]); }
+#pragma unroll
+                for (int k = 0; k < L; k++) {
+                    end = gate_a<SIGMOID>(v[k]) * (static_cast<double>(g[k]) + end);
+                    KTH_STEPS_APART(k);
+                }
+                slot[i * width].H = end;
+            }
+            __syncthreads();
+        }
+        hand_on_end(pl, w, before_tile, end);
+    } else {
+        K = state_before_wave<SIGMOID>(pl, w, K, lds);
+    }
 #pragma unroll
     for (int k = 0; k < L; k++) {
         if (q0 + k < pl.steps) {
@@ -461,8 +566,9 @@ struct NarrowPlace {
     uint32_t channel;                // of all, this thread's
 };
 
-__device__ __forceinline__ bool place_narrow(const NarrowPlan& pl, uint32_t* lds_ticket, NarrowPlace& w) {
+__device__ __forceinline__ bool place_narrow(const NarrowPlan& pl, uint32_t* lds_ticket, uint32_t* wild, NarrowPlace& w) {
     uint32_t ticket = blockIdx.x;
+    if (threadIdx.x == 0) *wild = 0;
     if (pl.tiles > 1) {
         if (threadIdx.x == 0) *lds_ticket = atomicAdd(pl.tickets, 1u);
         __syncthreads();
@@ -500,28 +606,30 @@ __device__ __forceinline__ uint64_t narrow_index(const NarrowPlan& pl, const Nar
     return (static_cast<uint64_t>(w.o0 + r) * pl.steps + first + t) * pl.inner + c;
 }
 
-// The state before this thread's piece from the piece's pair (A, H); `initial` is its channel's, read by the first piece of
-// the first tile. pair: kNarrowThreads pairs of LDS; handed: kSuper x inner more, and inner states.
-__device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, const NarrowPlace& w, double A, double H, double initial,
-                                                      Pair* pair, Pair* handed, double* carried) {
-    Pair mine = w.works ? Pair{A, H} : Pair{1.0, 0.0};
-    if (w.works && w.tile == 0 && w.j == 0) mine = Pair{0.0, advance(A, H, initial)};   // nobody else reads `initial`
+// The state before this thread's piece from the piece's pair and whether its steps are `tame`. `initial` is its channel's, read by
+// the first piece of the first tile. pair: kNarrowThreads pairs of LDS; handed: kSuper x inner more, and inner states; wild: 0
+// before the last barrier. in_turn: a piece of this tile is to be walked, so all are, one after another, and what is
+// returned is the state before the tile.
+template <bool SIGMOID>
+__device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, const NarrowPlace& w, const Pair& run, bool tame, double initial,
+                                                      Pair* pair, Pair* handed, double* carried, uint32_t* wild, bool& in_turn) {
+    Pair mine = w.works ? run : Pair{1.0, 0.0};
+    if (w.works && w.tile == 0 && w.j == 0) mine = Pair{0.0, advance<SIGMOID>(run, initial)};   // nobody else reads `initial`
     for (uint32_t d = 1; d < pl.pieces; d <<= 1) {                     // pieces up to and with this one
         pair[threadIdx.x] = mine;
         __syncthreads();
-        if (w.works && w.j >= d) {
-            const Pair p = pair[threadIdx.x - d * pl.inner];
-            mine = Pair{product(mine.A, p.A), advance(mine.A, mine.H, p.H)};
-        }
+        if (w.works && w.j >= d) mine = after<SIGMOID>(mine, pair[threadIdx.x - d * pl.inner]);
         __syncthreads();
     }
     pair[threadIdx.x] = mine;
+    if (!SIGMOID && w.works && (!tame || !(fabs(mine.A) < INFINITY))) *wild = 1;
     __syncthreads();
+    in_turn = !SIGMOID && __builtin_amdgcn_readfirstlane(*wild) != 0;
     double state = 0.0;
+    const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
     if (pl.tiles > 1) {
-        const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
         const Pair* total = pair + (pl.pieces - 1) * pl.inner;        // (a tile that is cut short is the last: nobody reads its total)
-        if (threadIdx.x < pl.inner && w.tile + 1 < pl.tiles && many + 1 < kSuper) {
+        if (threadIdx.x < pl.inner && w.tile + 1 < pl.tiles && many + 1 < kSuper && !in_turn) {
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.channels + w.o0 * pl.inner + threadIdx.x) * 2;
             publish(word, total[threadIdx.x].A, pl.tag);
             publish(word + 1, total[threadIdx.x].H, pl.tag);
@@ -537,19 +645,33 @@ __device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, cons
             if (threadIdx.x < pl.inner) {
                 const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
                 double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.tag, pl.lost);
-                for (uint32_t t = 0; t < many; t++) { const Pair p = handed[t * pl.inner + threadIdx.x]; s = advance(p.A, p.H, s); }
+                for (uint32_t t = 0; t < many; t++) s = advance<SIGMOID>(handed[t * pl.inner + threadIdx.x], s);
                 carried[threadIdx.x] = s;
-                if (many + 1 == kSuper && w.tile + 1 < pl.tiles)
-                    publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance(total[threadIdx.x].A, total[threadIdx.x].H, s), pl.tag);
+                if (many + 1 == kSuper && w.tile + 1 < pl.tiles && !in_turn)
+                    publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance<SIGMOID>(total[threadIdx.x], s), pl.tag);
             }
             __syncthreads();
             state = carried[w.c];
         }
     }
+    if (in_turn) return w.tile == 0 ? initial : state;
     if (w.tile == 0 && w.j == 0) return initial;
     if (w.j == 0) return state;
-    const Pair p = pair[threadIdx.x - pl.inner];
-    return advance(p.A, p.H, state);
+    return advance<SIGMOID>(pair[threadIdx.x - pl.inner], state);
+}
+// What a tile whose pieces took turns hands on; `before_tile` is that of thread i's channel i.
+__device__ __forceinline__ void narrow_hand_on_end(const NarrowPlan& pl, const NarrowPlace& w, double before_tile, const Pair* pair) {
+    if (threadIdx.x >= pl.inner || w.tile + 1 >= pl.tiles) return;
+    const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
+    const double end = pair[(pl.pieces - 1) * pl.inner + threadIdx.x].H;
+    if (w.tile % kSuper + 1 == kSuper) {
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.channels + channel, end, pl.tag);
+    } else {
+        uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.channels + channel) * 2;
+        const Pair total = known(before_tile, end);
+        publish(word, total.A, pl.tag);
+        publish(word + 1, total.H, pl.tag);
+    }
 }
 
 // LDS of both kernels: two stretches of floats, the pairs, what earlier tiles handed on.
@@ -558,7 +680,7 @@ struct NarrowShared {
     Pair   pair[kNarrowThreads];
     Pair   handed[kSuper * kNarrowInner];
     double carried[kNarrowInner];
-    uint32_t ticket;
+    uint32_t ticket, wild;
 };
 
 template <bool SIGMOID>
@@ -566,7 +688,7 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kern
                                                                                    float* __restrict__ out, float* final_state, NarrowPlan pl) {
     __shared__ NarrowShared sh;
     NarrowPlace w;
-    if (!place_narrow(pl, &sh.ticket, w)) return;
+    if (!place_narrow(pl, &sh.ticket, &sh.wild, w)) return;
     const uint32_t floats = w.rows * w.count * pl.inner;
 #pragma unroll 8
     for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
@@ -579,8 +701,8 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kern
     __syncthreads();
     const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
     const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
-    double A = 1.0, H = 0.0;
-    Least<SIGMOID> least;
+    double H = 0.0;
+    Product<SIGMOID> product;
     for (uint32_t k = 0; k < count; k++) {
         const uint32_t i = base + k * pl.inner;
         const float v = pack_gate<SIGMOID>(sh.a[i]);
@@ -588,10 +710,28 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_forward_narrow_kern
         if (SIGMOID) { sh.a[i] = v; sh.b[i] = u; }
         const double a = gate_a<SIGMOID>(v);
         H = fma(a, H, static_cast<double>(u));
-        A *= a;
-        least.take(v);
+        product.take(a, v, k);
     }
-    double h = narrow_state_before(pl, w, least.keep(A), H, start, sh.pair, sh.handed, sh.carried);
+    const Pair mine{product.gates(), H};
+    bool in_turn;
+    double h = narrow_state_before<SIGMOID>(pl, w, mine, product.tame(), start, sh.pair, sh.handed, sh.carried, &sh.wild, in_turn);
+    if (in_turn) {
+        const double before_tile = h;
+        float v[kSub], u[kSub];
+#pragma unroll
+        for (uint32_t k = 0; k < kSub; k++) if (k < count) { v[k] = sh.a[base + k * pl.inner]; u[k] = sh.b[base + k * pl.inner]; }
+        for (uint32_t j = 0; j < pl.pieces; j++) {
+            if (w.works && w.j == j) {
+                if (j > 0) h = sh.pair[threadIdx.x - pl.inner].H;
+                double end = h;
+#pragma unroll
+                for (uint32_t k = 0; k < kSub; k++) if (k < count) end = fma(gate_a<SIGMOID>(v[k]), end, static_cast<double>(u[k]));
+                sh.pair[threadIdx.x].H = end;
+            }
+            __syncthreads();
+        }
+        narrow_hand_on_end(pl, w, before_tile, sh.pair);
+    }
     for (uint32_t k = 0; k < count; k++) {
         const uint32_t i = base + k * pl.inner;
         h = fma(gate_a<SIGMOID>(sh.a[i]), h, static_cast<double>(sh.b[i]));
@@ -614,7 +754,7 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
                                                                                     float* __restrict__ grad_initial, NarrowPlan pl) {
     __shared__ NarrowShared sh;
     NarrowPlace w;
-    if (!place_narrow(pl, &sh.ticket, w)) return;
+    if (!place_narrow(pl, &sh.ticket, &sh.wild, w)) return;
     const uint32_t floats = w.rows * w.count * pl.inner;
 #pragma unroll 8
     for (uint32_t e = threadIdx.x; e < floats; e += kNarrowThreads) {
@@ -627,8 +767,8 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
     __syncthreads();
     const uint32_t base = (w.r * pl.pieces + w.j) * (kSub * pl.inner + 1) + w.c;
     const uint32_t count = w.works && w.j * kSub < w.count ? min(kSub, w.count - w.j * kSub) : 0;
-    double A = 1.0, H = 0.0;
-    Least<SIGMOID> least;
+    double H = 0.0;
+    Product<SIGMOID> product;
     float v[kSub], g[kSub];
 #pragma unroll
     for (uint32_t k = 0; k < kSub; k++) {
@@ -638,11 +778,26 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
             g[k] = sh.b[i];
             const double a = gate_a<SIGMOID>(v[k]);
             H = a * (static_cast<double>(g[k]) + H);
-            A *= a;
-            least.take(v[k]);
+            product.take(a, v[k], k);
         }
     }
-    double K = narrow_state_before(pl, w, least.keep(A), H, start, sh.pair, sh.handed, sh.carried);
+    const Pair mine{product.gates(), H};
+    bool in_turn;
+    double K = narrow_state_before<SIGMOID>(pl, w, mine, product.tame(), start, sh.pair, sh.handed, sh.carried, &sh.wild, in_turn);
+    if (in_turn) {
+        const double before_tile = K;
+        for (uint32_t j = 0; j < pl.pieces; j++) {
+            if (w.works && w.j == j) {
+                if (j > 0) K = sh.pair[threadIdx.x - pl.inner].H;
+                double end = K;
+#pragma unroll
+                for (uint32_t k = 0; k < kSub; k++) if (k < count) end = gate_a<SIGMOID>(v[k]) * (static_cast<double>(g[k]) + end);
+                sh.pair[threadIdx.x].H = end;
+            }
+            __syncthreads();
+        }
+        narrow_hand_on_end(pl, w, before_tile, sh.pair);
+    }
     __syncthreads();                                                   // gate and grad_out are in registers: their LDS is free
     if (grad_gate) {                                                   // (without it out and in need not be given)
 #pragma unroll 8
