@@ -405,8 +405,8 @@ int kth_dropout(uint64_t in, uint64_t n, double p, uint64_t seed, uint64_t offse
  * gates may decay and grow as they like: a state that falls below the range of a double is 0 from there on and one that
  * grows past it infinite or NaN, as step by step; one that falls by more than 2^1022 within a few hundred steps
  * counts as 0 already. Long sequences are cut into tiles that wait for one another inside the launch; should such a wait be given up (after seconds,
- * on a device that stands still), the results behind it are NaN and the next kth_sync, kth_download or kth_read_scalar
- * returns KTH_E_DEVICE. */
+ * on a device that stands still), the results behind it are NaN and the next kth_sync, kth_download, kth_read_scalar or
+ * kth_contains_nan returns KTH_E_DEVICE, once. */
 int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial,
                                  uint64_t out, uint64_t final_state);
 

@@ -1,5 +1,5 @@
 /*
- * kten_hip_bench.h — measurement entry points of libkten_hip.so that have no counterpart in the
+ * kten_hip_bench.h — entry points of libkten_hip.so for measurements and tests that have no counterpart in the
  * reference's backend contract (the reference has no timing facility). They are exported by the
  * same library as the entry points of kten_hip.h and are kept out of that header so that a host
  * binding the contract (the Kotlin HipRawTensor / HipTensorOperations pair) does not meet them:
@@ -49,6 +49,12 @@ int kth_profile_begin(void);
 int kth_profile_end(void);
 int kth_profile_count(int* count);
 int kth_profile_entry(int index, char* name, size_t cap, uint64_t* launches, uint64_t* bytes, double* total_ms);
+
+/* How often a tile of a gated recurrence looks for the state of the tiles before it until it gives up (kten_hip.h says what a
+ * caller sees then): 2^22 after kth_init. With 0 a tile gives up without a look, so that a test sees the same without a
+ * device that stands still: results from the second tile of a sequence on are NaN, and the next blocking call returns
+ * KTH_E_DEVICE. Holds for the calls that follow. */
+int kth_recurrence_wait_limit(uint32_t looks);
 
 #ifdef __cplusplus
 }

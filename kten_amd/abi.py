@@ -100,6 +100,7 @@ BENCH_SIGNATURES = {
     "kth_profile_end": (c_int, []),
     "kth_profile_count": (c_int, [POINTER(c_int)]),
     "kth_profile_entry": (c_int, [c_int, ctypes.c_char_p, c_size_t, POINTER(c_uint64), POINTER(c_uint64), POINTER(c_double)]),
+    "kth_recurrence_wait_limit": (c_int, [ctypes.c_uint32]),
 }
 
 _lib = None

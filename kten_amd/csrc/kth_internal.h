@@ -137,6 +137,7 @@ struct State {
     uint64_t* scan = nullptr;
     uint64_t  scan_words = 0;
     uint32_t  scan_tag = 0;
+    uint32_t  scan_polls = 1u << 22;            // kth_recurrence_wait_limit
     static constexpr int kScanLost = 16;        // the int behind host_index_flag that a recurrence sets if a wait was given up
 
     std::vector<hipEvent_t> laps;           // kth_timer_lap events not yet read by kth_timer_laps

@@ -163,14 +163,19 @@ __device__ __forceinline__ void publish(uint64_t* word, double v, uint32_t tag) 
     const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v)) + (1ull << (kTagBits - 1));
     __hip_atomic_store(word, (bits & ~static_cast<uint64_t>(kTags)) | tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// Waits for a word of an earlier tile. Should it not come within kMostPolls (seconds; a tile takes microseconds) the wave goes
-// on with NaN and leaves a mark for the host, which reports it at its next wait for the stream: no wait is endless.
-constexpr uint32_t kMostPolls = 1u << 22;
-__device__ __forceinline__ double await(const uint64_t* word, uint32_t tag, int* lost) {
-    uint64_t bits = __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (uint32_t polls = 0; (bits & kTags) != tag; polls++) {
-        if (polls == kMostPolls) {
-            __hip_atomic_store(lost, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+// Waits for a word of an earlier tile. Should it not come within `most` looks (the default takes seconds; a tile takes
+// microseconds) the wave goes on with NaN and leaves a mark for the host, which reports it at its next wait for the stream. Who
+// finds the mark while waiting, a look at the host's memory every thousand, gives up too: no wait is endless, nor is one given
+// up after another in a chain of tiles.
+struct Wait {
+    uint32_t tag, most;
+    int*     lost;                   // the host's word for a wait that was given up
+};
+__device__ __forceinline__ double await(const uint64_t* word, const Wait& wait) {
+    uint64_t bits = wait.most != 0 ? __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    for (uint32_t looks = 1; (bits & kTags) != wait.tag; looks++) {
+        if (looks >= wait.most || (looks % 1024 == 0 && __hip_atomic_load(wait.lost, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) != 0)) {
+            __hip_atomic_store(wait.lost, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
             return __builtin_nan("");
         }
         __builtin_amdgcn_s_sleep(1);
@@ -246,9 +251,8 @@ struct TilePlan {
     uint32_t tiles;                  // along the steps
     uint32_t cw, tw;                 // waves of a workgroup across channels and along steps
     uint32_t padded;                 // groups x cw x 64: channels with their padding
-    uint32_t tag;
+    Wait     wait;                   // with this launch's tag
     uint32_t* tickets;               // this launch's counter
-    int*      lost;                  // the host's word for a wait that was given up
     uint64_t* pairs;                 // [tiles][padded][2]
     uint64_t* states;                // [tiles / kSuper][padded]
     FastDiv  group_div, col_div;
@@ -309,8 +313,8 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
             for (uint32_t i = 1; i < pl.tw; i++) total = after<SIGMOID>(lds[i * width + at], total);
             if (w.tile == 0) total = Pair{0.0, advance<SIGMOID>(total, initial)};     // nobody else reads `initial`
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
-            publish(word, total.A, pl.tag);
-            publish(word + 1, total.H, pl.tag);
+            publish(word, total.A, pl.wait.tag);
+            publish(word + 1, total.H, pl.wait.tag);
         }
         if (w.tile > 0) {
             // the waves along the steps share out the tiles before
@@ -319,11 +323,11 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
             Pair p{1.0, 0.0};
             for (uint32_t i = from; i < to; i++) {
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + i) * pl.padded + w.slot) * 2;
-                const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
+                const double a = await(word, pl.wait), h = await(word + 1, pl.wait);
                 p = after<SIGMOID>(Pair{a, h}, p);
             }
             before[w.twi * width + at] = p;
-            state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.tag, pl.lost);
+            state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.wait);
             __syncthreads();
             for (uint32_t i = 0; i < pl.tw; i++) state = advance<SIGMOID>(before[i * width + at], state);
         }
@@ -337,7 +341,7 @@ __device__ __forceinline__ double state_before_wave(const TilePlan& pl, const Ti
     if (w.twi == pl.tw - 1 && w.tile % kSuper + 1 == kSuper && w.tile + 1 < pl.tiles) {
         double end = state;
         for (uint32_t i = 0; i < pl.tw; i++) end = advance<SIGMOID>(lds[i * width + at], end);
-        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.tag);
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.wait.tag);
     }
     for (uint32_t i = 0; i < w.twi; i++) state = advance<SIGMOID>(lds[i * width + at], state);
     return state;
@@ -346,12 +350,12 @@ __device__ __forceinline__ double state_before_wave(const TilePlan& pl, const Ti
 __device__ __forceinline__ void hand_on_end(const TilePlan& pl, const TilePlace& w, double before_tile, double end) {
     if (w.twi != pl.tw - 1 || w.tile + 1 >= pl.tiles) return;
     if (w.tile % kSuper + 1 == kSuper) {
-        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.tag);
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.wait.tag);
     } else {
         uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
         const Pair total = known(before_tile, end);
-        publish(word, total.A, pl.tag);
-        publish(word + 1, total.H, pl.tag);
+        publish(word, total.A, pl.wait.tag);
+        publish(word + 1, total.H, pl.wait.tag);
     }
 }
 
@@ -550,9 +554,8 @@ struct NarrowPlan {
     uint32_t pieces;                 // of kSub steps, of a row in a workgroup
     uint32_t tile_steps, tiles;
     uint32_t channels;               // outer x inner
-    uint32_t tag;
+    Wait     wait;                   // with this launch's tag
     uint32_t* tickets;               // this launch's counter
-    int*      lost;                  // the host's word for a wait that was given up
     uint64_t* pairs;                 // [tiles][channels][2]
     uint64_t* states;                // [tiles / kSuper][channels]
     FastDiv  inner_div, row_div, outer_div, piece_div;     // row_div divides by the floats of a row of this workgroup
@@ -631,24 +634,24 @@ __device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, cons
         const Pair* total = pair + (pl.pieces - 1) * pl.inner;        // (a tile that is cut short is the last: nobody reads its total)
         if (threadIdx.x < pl.inner && w.tile + 1 < pl.tiles && many + 1 < kSuper && !in_turn) {
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.channels + w.o0 * pl.inner + threadIdx.x) * 2;
-            publish(word, total[threadIdx.x].A, pl.tag);
-            publish(word + 1, total[threadIdx.x].H, pl.tag);
+            publish(word, total[threadIdx.x].A, pl.wait.tag);
+            publish(word + 1, total[threadIdx.x].H, pl.wait.tag);
         }
         if (w.tile > 0) {
             for (uint32_t i = threadIdx.x; i < many * pl.inner; i += kNarrowThreads) {
                 const uint32_t t = divide(i, pl.inner_div);
                 const uint64_t* word = pl.pairs + (static_cast<uint64_t>(first + t) * pl.channels + w.o0 * pl.inner + (i - t * pl.inner)) * 2;
-                const double a = await(word, pl.tag, pl.lost), h = await(word + 1, pl.tag, pl.lost);
+                const double a = await(word, pl.wait), h = await(word + 1, pl.wait);
                 handed[i] = Pair{a, h};
             }
             __syncthreads();
             if (threadIdx.x < pl.inner) {
                 const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
-                double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.tag, pl.lost);
+                double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.wait);
                 for (uint32_t t = 0; t < many; t++) s = advance<SIGMOID>(handed[t * pl.inner + threadIdx.x], s);
                 carried[threadIdx.x] = s;
                 if (many + 1 == kSuper && w.tile + 1 < pl.tiles && !in_turn)
-                    publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance<SIGMOID>(total[threadIdx.x], s), pl.tag);
+                    publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance<SIGMOID>(total[threadIdx.x], s), pl.wait.tag);
             }
             __syncthreads();
             state = carried[w.c];
@@ -665,12 +668,12 @@ __device__ __forceinline__ void narrow_hand_on_end(const NarrowPlan& pl, const N
     const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
     const double end = pair[(pl.pieces - 1) * pl.inner + threadIdx.x].H;
     if (w.tile % kSuper + 1 == kSuper) {
-        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.channels + channel, end, pl.tag);
+        publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.channels + channel, end, pl.wait.tag);
     } else {
         uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.channels + channel) * 2;
         const Pair total = known(before_tile, end);
-        publish(word, total.A, pl.tag);
-        publish(word + 1, total.H, pl.tag);
+        publish(word, total.A, pl.wait.tag);
+        publish(word + 1, total.H, pl.wait.tag);
     }
 }
 
@@ -857,7 +860,7 @@ Path path_of(const ScanShape& sh, bool forward) {
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
 // one stream, and each has a tag and a counter of its own.
-int take_words(const char* what, uint64_t words, uint32_t* tag, uint32_t** counter, uint64_t** first, int** lost) {
+int take_words(const char* what, uint64_t words, Wait* wait, uint32_t** counter, uint64_t** first) {
     constexpr uint64_t kHead = (kTags + 1) / 2;              // every tag's counter
     State& s = state();
     words += kHead;
@@ -880,10 +883,9 @@ int take_words(const char* what, uint64_t words, uint32_t* tag, uint32_t** count
         s.scan_tag = 0;
     }
     s.scan_tag += 1;
-    *tag = s.scan_tag;
+    *wait = Wait{s.scan_tag, s.scan_polls, s.host_index_flag_device + State::kScanLost};
     *counter = reinterpret_cast<uint32_t*>(s.scan) + s.scan_tag;
     *first = s.scan + kHead;
-    *lost = s.host_index_flag_device + State::kScanLost;
     return KTH_OK;
 }
 
@@ -899,7 +901,7 @@ int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     pl.col_div = make_div(pl.col_blocks);
     if (pl.tiles > 1) {
         const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.padded * 2;
-        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded, &pl.tag, &pl.tickets, &pl.pairs, &pl.lost)) return rc;
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.padded, &pl.wait, &pl.tickets, &pl.pairs)) return rc;
         pl.states = pl.pairs + pairs;
     }
     *out = pl;
@@ -923,7 +925,7 @@ int plan_narrow(const char* what, const ScanShape& sh, NarrowPlan* out, uint32_t
     *grid = pl.tiles > 1 ? pl.tiles * sh.outer : (sh.outer - 1) / pl.rows + 1;
     if (pl.tiles > 1) {
         const uint64_t pairs = static_cast<uint64_t>(pl.tiles) * pl.channels * 2;
-        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.channels, &pl.tag, &pl.tickets, &pl.pairs, &pl.lost))
+        if (int rc = take_words(what, pairs + static_cast<uint64_t>(pl.tiles / kSuper) * pl.channels, &pl.wait, &pl.tickets, &pl.pairs))
             return rc;
         pl.states = pl.pairs + pairs;
     }
@@ -958,6 +960,13 @@ int shape_of(const char* what, const int32_t* shape, int dims, int axis, int mod
 }  // namespace
 
 extern "C" {
+
+int kth_recurrence_wait_limit(uint32_t looks) {
+    std::lock_guard<std::mutex> guard(lock());
+    KTH_REQUIRE_INIT();
+    state().scan_polls = looks;
+    return KTH_OK;
+}
 
 int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial,
                                  uint64_t out, uint64_t final_state) {
