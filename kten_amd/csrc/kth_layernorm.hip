@@ -6,7 +6,7 @@
 //   backward   xh = (x - m) r,  w = go gamma:   gin = r (w - mean(w) - xh mean(w xh)),
 //              grad_gamma = sum over rows of go xh,  grad_beta = sum over rows of go
 //
-// Every sum is made in f64 from d = x - k with k the row's first element (as the batch norm kernels do): the sums of d and
+// Every sum is made in f64 from d = x - k with k the row's first element (0 if that is not finite): the sums of d and
 // d^2 then give the mean and the variance in one pass, at a cancellation of at most n 2^-53 of the spread around k; the
 // backward pass takes the sums of w and w d along and works the statistics out again, so that it needs nothing saved.
 // Sums are folded in a fixed order: the same input gives the same bits.
@@ -49,6 +49,10 @@ __device__ __forceinline__ double row_rstd(double v, double eps) {
 __device__ __forceinline__ float ln_forward(float x, double mean, double rstd, float gamma, float beta) {
     return static_cast<float>((static_cast<double>(x) - mean) * rstd) * gamma + beta;
 }
+
+// The value k that a row's sums are made around, from the row's first: around an infinity the sums would lose the mean. (Where
+// lanes behind the last column have that infinity for their values, the row's sum has it already.)
+__device__ __forceinline__ float around(float first) { return fabsf(first) < INFINITY ? first : 0.0f; }
 
 // Sums of NS doubles over a workgroup of kBlock threads; every thread of wave 0 returns them.
 template <int NS>
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(ForwardGroup<G>::threads) void ln_forward_rows_kern
         float v[U][4];
 #pragma unroll
         for (int u = 0; u < U; u++) load4<false>(x + at, (u * G + lane) * 4, sh.cols, first, v[u]);
-        const double k = static_cast<double>(first);
+        const double k = static_cast<double>(around(first));
         double s[2] = {};
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(kLongThreads) void ln_forward_long_kernel(const flo
     for (uint32_t row = blockIdx.x; row < sh.rows; row += gridDim.x) {
         const uint64_t at = static_cast<uint64_t>(row) * sh.cols;
         const float first = x[at];
-        const double k = static_cast<double>(first);
+        const double k = static_cast<double>(around(first));
         double s[2] = {};
         v4f_any v[R > 0 ? R : 1];                            // (columns that every such row has)
 #pragma unroll
@@ -431,7 +435,7 @@ __global__ __launch_bounds__(kBlock) void ln_sums_kernel(const float* __restrict
     const float* gr = BACKWARD ? go + static_cast<uint64_t>(row) * pl.sh.cols : nullptr;
     const uint32_t first = seg * pl.seg_len;
     const uint32_t last = min(first + pl.seg_len, pl.sh.cols);
-    const double k = static_cast<double>(xr[0]);
+    const double k = static_cast<double>(around(xr[0]));
     double s[NS] = {};
     auto add = [&](float xv, float gv, float ga) {
         const double d = static_cast<double>(xv) - k;
@@ -510,7 +514,7 @@ __global__ __launch_bounds__(kBlock) void ln_rows_kernel(const float* __restrict
     if ((threadIdx.x & 63) != 0) return;
     const double inv = pl.sh.inv_cols;
     const double delta = s[0] * inv;
-    const double mean = static_cast<double>(x[static_cast<uint64_t>(row) * pl.sh.cols]) + delta;
+    const double mean = static_cast<double>(around(x[static_cast<uint64_t>(row) * pl.sh.cols])) + delta;
     const double rstd = row_rstd(row_variance(s[0], s[1], inv), eps);
     if (BACKWARD) {
         bwd[row] = RowBackward{mean, rstd, s[NS - 2] * inv, (s[NS - 1] - delta * s[NS - 2]) * rstd * rstd * inv};
