@@ -143,7 +143,7 @@ __device__ __forceinline__ void row_fold(double (&s)[NS], double* lds, uint32_t&
 // 1 / sqrt(v + eps) in f64: the hardware's estimate (24 bits) and one Newton step.
 __device__ __forceinline__ double row_rstd_fast(double v, double eps) {
     const double s = v + eps;
-    if (s == 0.0) return 0.0;
+    if (s == 0.0 || s == INFINITY) return 0.0;         // (an infinite epsilon: the step would make NaN of it)
     const double y = __builtin_amdgcn_rsq(s);
     return fma(0.5 * y, fma(-s * y, y, 1.0), y);
 }

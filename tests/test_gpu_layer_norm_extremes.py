@@ -1,5 +1,5 @@
-"""Layer norm where a row's infinity comes first, last or between: the
-definition's mean, the same from each of its kernels."""
+"""Layer norm where a row's infinity comes first, last or between, and with an epsilon that swallows every variance: the
+definition's results, the same from each of its kernels."""
 import numpy as np
 import pytest
 
@@ -33,3 +33,17 @@ def test_mean_of_a_row_with_infinities(cols, gc):
     for row in (0, 7, 8):
         for a, b in zip(got, clean):
             assert_bits_equal(a[row:row + 1], b[row:row + 1], "the other rows")
+
+
+@pytest.mark.parametrize("cols", COLS)
+def test_infinite_epsilon(cols, gc):
+    """1 / sqrt(var + inf) is 0: the result is beta, and nothing of the gradient but beta's is left."""
+    x, gamma, beta, go = data(1, 5, cols), data(2, cols), data(3, cols), data(4, 5, cols)
+    raw = [gc.createRaw(list(a.shape), a) for a in (x, gamma, beta, go)]
+    norm = gc.layerNorm(1, np.inf)
+    out, _, std = norm.calculateOutput(raw[0], raw[1], raw[2])
+    assert (std.toArray() == 0).all()
+    assert (out.toArray() == np.broadcast_to(beta, x.shape)).all()
+    grad_in, grad_gamma, grad_beta = norm.calculateGrads(raw[0], raw[1], raw[3])
+    assert (grad_in.toArray() == 0).all() and (grad_gamma.toArray() == 0).all()
+    ref.assert_within(grad_beta.toArray(), ref.f64(go).sum(0), 3 * ref.U * np.abs(ref.f64(go)).sum(0), "grad of beta")
