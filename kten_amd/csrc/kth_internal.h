@@ -133,7 +133,8 @@ struct State {
     int*          host_index_flag_device = nullptr;
     IndexUse      index_use;
 
-    // what the tiles of a recurrence hand on through (kth_recurrence.hip): words, the last launch's tag
+    // what the tiles of a recurrence hand on through (kth_recurrence.hip): words, the last launch's tag. Kept between calls
+    // as buffers of the pool are, counted and given up with them.
     uint64_t* scan = nullptr;
     uint64_t  scan_words = 0;
     uint32_t  scan_tag = 0;
@@ -218,6 +219,9 @@ private:
 // later launch because every launch is on the one in-order stream.
 float* workspace_acquire(uint64_t bytes, uint64_t* cap_bytes);
 void   workspace_release(float* p, uint64_t cap_bytes);
+// State::scan with room for so many words, their contents unknown; the one before goes back to the pool. False if there is no
+// memory (State::scan is null then).
+bool scan_reserve(uint64_t words);
 
 // The ascending positions i in [0, n) with flags[i] != 0 and their number, on `stream` (kth_sort.hip).
 // With temp == nullptr only *temp_bytes is set, to the scratch size needed.

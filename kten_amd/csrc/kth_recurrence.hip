@@ -859,25 +859,14 @@ Path path_of(const ScanShape& sh, bool forward) {
 }
 
 // The words that tiles publish through live in memory of the library's own, kept between calls: calls follow one another on
-// one stream, and each has a tag and a counter of its own.
+// one stream, and each has a tag and a counter of its own. (Nothing that may take memory comes between this and the launch.)
 int take_words(const char* what, uint64_t words, Wait* wait, uint32_t** counter, uint64_t** first) {
     constexpr uint64_t kHead = (kTags + 1) / 2;              // every tag's counter
     State& s = state();
     words += kHead;
     if (words > s.scan_words || s.scan_tag == kTags) {
-        if (words > s.scan_words) {
-            KTH_HIP(hipStreamSynchronize(s.stream));
-            if (s.scan) KTH_HIP(hipFree(s.scan));
-            s.scan = nullptr; s.scan_words = 0;
-            const OnDevice here;
-            void* p = nullptr;
-            if (hipMalloc(&p, words * 8) != hipSuccess) {
-                (void)hipGetLastError();
-                return fail(KTH_E_MEMORY, "%s: no workspace of %llu bytes", what, static_cast<unsigned long long>(words * 8));
-            }
-            s.scan = static_cast<uint64_t*>(p);
-            s.scan_words = words;
-        }
+        if (words > s.scan_words && !scan_reserve(words))
+            return fail(KTH_E_MEMORY, "%s: no workspace of %llu bytes", what, static_cast<unsigned long long>(words * 8));
         for (uint64_t at = 0; at < s.scan_words; at += 1ull << 29)
             launch_fill(reinterpret_cast<float*>(s.scan + at), 2 * std::min<uint64_t>(s.scan_words - at, 1ull << 29), 0.0f);
         s.scan_tag = 0;

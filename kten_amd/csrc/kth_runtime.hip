@@ -234,6 +234,11 @@ static void trim_pool() {
         kv.second.clear();
     }
     s.pool.clear();
+    if (s.scan) {
+        (void)hipFree(s.scan);
+        s.pool_bytes -= s.scan_words * 8;
+        s.scan = nullptr; s.scan_words = 0;
+    }
 }
 
 static float* pool_take(uint64_t cap) {
@@ -271,6 +276,18 @@ float* workspace_acquire(uint64_t bytes, uint64_t* cap_bytes) {
     float* p = pool_take(cap);
     if (p) { *cap_bytes = cap; state().live_bytes += cap; }
     return p;
+}
+
+bool scan_reserve(uint64_t words) {
+    State& s = state();
+    if (s.scan) s.pool[s.scan_words * 8].push_back(reinterpret_cast<float*>(s.scan));
+    s.scan = nullptr; s.scan_words = 0;
+    const uint64_t cap = size_class(words * 8);
+    s.scan = reinterpret_cast<uint64_t*>(pool_take(cap));
+    if (!s.scan) return false;
+    s.scan_words = cap / 8;
+    s.pool_bytes += cap;
+    return true;
 }
 
 void workspace_release(float* p, uint64_t cap_bytes) {
@@ -357,7 +374,6 @@ static void teardown() {
     s.free_slots.clear();
     trim_pool();
     if (s.deferred_index_flag) (void)hipFree(s.deferred_index_flag);
-    if (s.scan) (void)hipFree(s.scan);
     if (s.host_index_flag) (void)hipHostFree(const_cast<int*>(s.host_index_flag));
     s.host_index_flag = nullptr; s.host_index_flag_device = nullptr;
     for (LaunchRecord& r : s.records) { (void)hipEventDestroy(r.begin); (void)hipEventDestroy(r.end); }
