@@ -96,6 +96,7 @@ int kth_dropout(uint64_t in, uint64_t n, double p, uint64_t seed, uint64_t offse
     Operand ops[3] = {{"in", in, n, false}, {"residual", residual, n, false}, {"out", out, n, true}};
     if (int rc = resolve_operands("kth_dropout", ops, 3, {{2, 0}, {2, 1}}, KTH_E_ARGUMENT)) return rc;
     if (n == 0) return KTH_OK;
+    overwrite_results(ops, 3);
     const float* sr = ops[1].ptr;
     DropoutPlan pl{};
     pl.seed = seed; pl.offset = offset;

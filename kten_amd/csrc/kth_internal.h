@@ -199,8 +199,10 @@ struct Operand {
 };
 // Looks the operands up. Everything is checked before anything is launched: handles, sizes (size_code where a store is too
 // small), and that no result shares its store with another operand but for the `allowed` pairs (result, other). Then what
-// the inputs are owed is launched, and what the results are owed dropped or launched.
+// the inputs are owed is launched. The results keep what they are owed, for the call may still be refused, until
+// overwrite_results, ahead of the launch that writes them, which drops or launches it.
 int resolve_operands(const char* what, Operand* ops, int count, std::initializer_list<std::pair<int, int>> allowed, int size_code = KTH_E_SHAPE);
+void overwrite_results(Operand* ops, int count);
 
 // Makes the library's device the calling thread's current one for a while: memory is allocated on the current device, and
 // a host's thread may have chosen another, or none yet.

@@ -783,6 +783,7 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
     float* const pout = ops[3].ptr; float* const pmean = ops[4].ptr; float* const pstd = ops[5].ptr;
 
     if (sh.cols <= kForwardRowCols) {
+        overwrite_results(ops, 6);
         LaunchScope scope("ln_forward_rows_kernel", "", n * 8);
         const ForwardRows k = forward_rows_kernel(sh);
         hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pga, pbe, pout, pmean, pstd, sh, static_cast<double>(epsilon));
@@ -790,6 +791,7 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
         return KTH_OK;
     }
     if (sh.cols <= (sh.rows >= kLongRows ? kLongRowCols : kLdsRowFloats) && long_rows_allowed()) {
+        overwrite_results(ops, 6);
         LaunchScope scope("ln_forward_long_kernel", "", n * 8);
         const bool lds_alone = sh.cols <= kLdsRowFloats;
         const uint32_t held = lds_alone ? sh.cols : sh.cols - kLongRegisters * kLongThreads * 4;
@@ -807,6 +809,7 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
     uint64_t cap;
     char* ws = reinterpret_cast<char*>(workspace_acquire(ws_bytes, &cap));
     if (!ws) return fail(KTH_E_MEMORY, "kth_layer_norm_forward: no workspace of %llu bytes", static_cast<unsigned long long>(ws_bytes));
+    overwrite_results(ops, 6);
     RowForward* rows = reinterpret_cast<RowForward*>(ws);
     double* partial = reinterpret_cast<double*>(ws + rows_bytes);
     hipStream_t stream = state().stream;
@@ -850,6 +853,7 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
         uint64_t part_cap = 0;
         float* part = part_bytes ? workspace_acquire(part_bytes, &part_cap) : nullptr;
         if (part_bytes && !part) return fail(KTH_E_MEMORY, "kth_layer_norm_backward: no workspace of %llu bytes", static_cast<unsigned long long>(part_bytes));
+        overwrite_results(ops, 6);
         {
             LaunchScope scope("ln_backward_rows_kernel", "", n * (pgi ? 12 : 8) + part_bytes);
             hipLaunchKernelGGL(k.kernel, dim3(k.grid), dim3(k.threads), 0, state().stream, px, pgo, pga, pgi, part, part ? nullptr : pgg, part ? nullptr : pgb, sh, static_cast<double>(epsilon));
@@ -879,6 +883,7 @@ int kth_layer_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
     uint64_t cap;
     char* ws = reinterpret_cast<char*>(workspace_acquire(ws_bytes, &cap));
     if (!ws) return fail(KTH_E_MEMORY, "kth_layer_norm_backward: no workspace of %llu bytes", static_cast<unsigned long long>(ws_bytes));
+    overwrite_results(ops, 6);
     RowBackward* rows = reinterpret_cast<RowBackward*>(ws);
     double* sums = reinterpret_cast<double*>(ws + rows_bytes);
     float* partial = weights ? reinterpret_cast<float*>(ws + rows_bytes + sums_bytes) : nullptr;

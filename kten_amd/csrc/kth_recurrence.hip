@@ -973,6 +973,7 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
     if (path == Path::narrow) {
         NarrowPlan pl; uint32_t grid;
         if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
+        overwrite_results(ops, 5);
         LaunchScope scope("recurrence_forward_narrow_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
         auto* kernel = sigmoid ? recurrence_forward_narrow_kernel<true> : recurrence_forward_narrow_kernel<false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr, pl);
@@ -983,6 +984,7 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         constexpr int L = 32;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
+        overwrite_results(ops, 5);
         LaunchScope scope("recurrence_forward_tiles_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
         const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
         const bool lines = sh.inner % 32 == 0;
@@ -992,6 +994,7 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         KTH_LAUNCH_CHECK("gated_recurrence_forward");
         return KTH_OK;
     }
+    overwrite_results(ops, 5);
     LaunchScope scope("recurrence_forward_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);
     if (sigmoid)
@@ -1024,6 +1027,7 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
     if (path == Path::narrow) {
         NarrowPlan pl; uint32_t grid;
         if (int rc = plan_narrow(what, sh, &pl, &grid)) return rc;
+        overwrite_results(ops, 9);
         LaunchScope scope("recurrence_backward_narrow_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
         auto* kernel = sigmoid ? recurrence_backward_narrow_kernel<true> : recurrence_backward_narrow_kernel<false>;
         hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNarrowThreads), 0, state().stream, ops[0].ptr, ops[1].ptr, ops[2].ptr, ops[3].ptr, ops[4].ptr,
@@ -1035,6 +1039,7 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
         constexpr int L = 16;
         TilePlan pl;
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
+        overwrite_results(ops, 9);
         LaunchScope scope("recurrence_backward_tiles_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
         const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
         const bool lines = sh.inner % 32 == 0;
@@ -1045,6 +1050,7 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
         KTH_LAUNCH_CHECK("gated_recurrence_backward");
         return KTH_OK;
     }
+    overwrite_results(ops, 9);
     LaunchScope scope("recurrence_backward_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
     const dim3 grid((sh.channels - 1) / kBlock + 1);
     if (sigmoid)

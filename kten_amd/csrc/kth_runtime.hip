@@ -206,12 +206,14 @@ int resolve_operands(const char* what, Operand* ops, int count, std::initializer
         if (ops[i].store && ops[i].result) (void)lookup_unsettled(ops[i].handle, what);
     for (int i = 0; i < count; i++)
         if (ops[i].store && !ops[i].result) (void)lookup(ops[i].handle, what, true);
-    for (int i = 0; i < count; i++) {
-        if (!ops[i].store) continue;
-        if (ops[i].result && ops[i].n != 0) settle_for_overwrite(ops[i].store, ops[i].n);      // (one that is an input too owes nothing any more)
-        ops[i].ptr = ops[i].store->ptr;
-    }
+    for (int i = 0; i < count; i++)
+        if (ops[i].store) ops[i].ptr = ops[i].store->ptr;
     return KTH_OK;
+}
+
+void overwrite_results(Operand* ops, int count) {
+    for (int i = 0; i < count; i++)
+        if (ops[i].store && ops[i].result && ops[i].n != 0) settle_for_overwrite(ops[i].store, ops[i].n);      // (one that is an input too owes nothing any more)
 }
 
 // Size classes: 512-byte granules up to 1 MiB, then 1/8-octave steps (at most 12.5 %

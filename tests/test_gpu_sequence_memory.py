@@ -47,6 +47,36 @@ CASES = {
         assert right(out)
         assert held() >= before + 4 * 1000 * 1000, (before, held())
     """,
+    "refused without room, and nothing of the result touched": """
+        out, grads = ops.createRawFill([N], 9.0), [ops.createRawFill([N], 9.0) for _ in range(2)]
+        budget(ops.getMetrics()["liveBytes"] + 64 * 1024)
+        launches = ops.getMetrics()["launches"]
+        assert forward(gate, x, out) == abi.KTH_E_MEMORY
+        assert lib.kth_gated_recurrence_backward(h(gate), 0, SHAPE, 3, 1, abi.KTH_GATE_GIVEN, 0, h(x), h(x), 0, h(grads[0]), h(grads[1]), 0) == abi.KTH_E_MEMORY
+        for t in [out] + grads:
+            assert (t.toArray() == 9.0).all()
+        budget(0.5 * total.value)
+        abi.check(forward(gate, x, out))
+        assert right(out)
+    """,
+    "a layer norm without its workspace": """
+        rows, cols = 8, 200000
+        a = ops.createRaw([rows, cols], np.random.default_rng(1).standard_normal(rows * cols).astype(np.float32))
+        go = a.copy(); go.toArray()
+        results = [ops.createRawFill([rows, cols], 9.0), ops.createRawFill([cols], 9.0), ops.createRawFill([cols], 9.0)]
+        out, mean, std = ops.createRawFill([rows, cols], 9.0), ops.createRawFill([rows], 9.0), ops.createRawFill([rows], 9.0)
+        shape = abi.shape_array([rows, cols])
+        def backward():
+            return lib.kth_layer_norm_backward(h(a), shape, 2, 1, 1e-5, 0, h(go), *(h(t) for t in results))
+        budget(ops.getMetrics()["liveBytes"])
+        assert backward() == abi.KTH_E_MEMORY
+        assert lib.kth_layer_norm_forward(h(a), shape, 2, 1, 1e-5, 0, 0, h(out), h(mean), h(std)) == abi.KTH_E_MEMORY
+        for t in results + [out, mean, std]:
+            assert (t.toArray() == 9.0).all()
+        budget(0.5 * total.value)
+        abi.check(backward())
+        assert np.isfinite(results[0].toArray()).all() and (results[2].toArray() != 9.0).all()
+    """,
     "room is made from the pool, and the words are given up for a store": """
         out = ops.createRaw([N])
         parked = ops.createRaw([16 * MIB // 4]); parked.release()        # 16 MiB that nobody uses
