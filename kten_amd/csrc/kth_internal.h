@@ -133,6 +133,8 @@ struct State {
     int*          host_index_flag_device = nullptr;
     IndexUse      index_use;
 
+    bool long_rows = false;                 // layer_norm_init: the device grants the LDS of the kernel for long rows
+
     // what the tiles of a recurrence hand on through (kth_recurrence.hip): words, the last launch's tag. Kept between calls
     // as buffers of the pool are, counted and given up with them.
     uint64_t* scan = nullptr;
@@ -242,6 +244,10 @@ hipError_t sort_pairs_u32(void* temp, size_t* temp_bytes, const uint32_t* keys_i
 // Resolves the device address of the static scratch array of kth_reduce_axis_static for
 // `device`, which must be the current device (kth_reduce.hip). Called once from kth_init.
 hipError_t reduce_scratch_init(int device);
+
+// Whether the current device grants the LDS that layer norm's kernel for long rows asks for (kth_layernorm.hip). Called from
+// every kth_init: what was granted holds for the device of a session, not for the next one's.
+bool layer_norm_init();
 
 // In deferred index checking: reads and clears the persistent flag (the stream must be drained) and returns
 // KTH_E_ARGUMENT if an indexed move since the last report met an index outside its axis, KTH_OK otherwise.

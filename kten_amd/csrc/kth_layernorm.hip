@@ -717,19 +717,6 @@ ForwardRows forward_rows_kernel(const Shape2& sh) {
          : c <= 8192 ? forward_rows_of<512, 4>(sh, 2) : forward_rows_of<1024, 4>(sh, 1);
 }
 
-// A workgroup may use 64 KiB of dynamic LDS unless the kernel is granted more.
-bool long_rows_allowed() {
-    static const bool allowed = [] {
-        const OnDevice here;
-        bool ok = true;
-        for (const void* f : {reinterpret_cast<const void*>(&ln_forward_long_kernel<0>), reinterpret_cast<const void*>(&ln_forward_long_kernel<kLongRegisters>)})
-            ok = ok && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsRowFloats * 4) == hipSuccess;
-        if (!ok) (void)hipGetLastError();
-        return ok;
-    }();
-    return allowed;
-}
-
 struct BackwardRows {
     void (*kernel)(const float*, const float*, const float*, float*, float*, float*, float*, Shape2, double);
     uint32_t threads, grid;
@@ -766,6 +753,15 @@ uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
 
 }  // namespace
 
+// A workgroup may use 64 KiB of dynamic LDS unless the kernel is granted more.
+bool kth::layer_norm_init() {
+    bool ok = true;
+    for (const void* f : {reinterpret_cast<const void*>(&ln_forward_long_kernel<0>), reinterpret_cast<const void*>(&ln_forward_long_kernel<kLongRegisters>)})
+        ok = ok && hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsRowFloats * 4) == hipSuccess;
+    if (!ok) (void)hipGetLastError();
+    return ok;
+}
+
 extern "C" {
 
 int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis, float epsilon, uint64_t gamma, uint64_t beta,
@@ -790,7 +786,7 @@ int kth_layer_norm_forward(uint64_t in, const int32_t* shape, int dims, int axis
         KTH_LAUNCH_CHECK("layer_norm_forward");
         return KTH_OK;
     }
-    if (sh.cols <= (sh.rows >= kLongRows ? kLongRowCols : kLdsRowFloats) && long_rows_allowed()) {
+    if (sh.cols <= (sh.rows >= kLongRows ? kLongRowCols : kLdsRowFloats) && state().long_rows) {
         overwrite_results(ops, 6);
         LaunchScope scope("ln_forward_long_kernel", "", n * 8);
         const bool lds_alone = sh.cols <= kLdsRowFloats;

@@ -399,6 +399,7 @@ static int bring_up(int device) {
     KTH_HIP(hipEventCreate(&s.ev_end));
     KTH_HIP(init_math_tables());
     KTH_HIP(reduce_scratch_init(device));
+    s.long_rows = layer_norm_init();
     KTH_HIP(hipMalloc(reinterpret_cast<void**>(&s.deferred_index_flag), 256));
     KTH_HIP(hipMemset(s.deferred_index_flag, 0, 256));
     void* host = nullptr; void* dev = nullptr;
