@@ -269,6 +269,7 @@ public:
             : axis_(axis), mode_(sigmoidGate ? KTH_GATE_SIGMOID : KTH_GATE_GIVEN), ops_(ops) {}
         RecurrenceOutputs calculateOutput(const Raw& gate, const Raw& input, const Raw& initial);
         Raw step(const Raw& gate, const Raw& input, const Raw& state);          // `state` is updated in place
+        // input, initial and output are read for the gate's gradient only, input only with sigmoidGate: null where they are not
         RecurrenceGrads calculateGrads(const Raw& gate, const Raw& input, const Raw& initial, const Raw& output, const Raw& gradOut,
                                        const Raw& gradFinal, bool gateRequiresGrad, bool inRequiresGrad, bool initialRequiresGrad);
     private:
@@ -800,11 +801,11 @@ inline Raw HipTensorOperations::Dropout::calculateOutput(const Raw& input, const
     return r;
 }
 inline Shape HipTensorOperations::GatedRecurrence::stateShape(const Raw& gate, const Raw& input, const Raw& initial, int* axis) const {
-    if (gate->shape != input->shape)
+    if (input && gate->shape != input->shape)
         throw std::invalid_argument("Gate and input of a recurrence must have the same shape, got " + to_string(gate->shape) + " and " +
                                     to_string(input->shape));
-    *axis = normalizeAxis(input->shape, axis_);
-    Shape state = input->shape;
+    *axis = normalizeAxis(gate->shape, axis_);
+    Shape state = gate->shape;
     state.erase(state.begin() + *axis);
     detail::requireSize("The initial state of a recurrence", initial, toStoreSize(state));
     return detail::orOne(state);
@@ -814,8 +815,8 @@ inline HipTensorOperations::RecurrenceOutputs HipTensorOperations::GatedRecurren
     const uint64_t g = handleOf(gate), in = handleOf(input), h0 = handleOf(initial);
     int axis = 0;
     const Shape state = stateShape(gate, input, initial, &axis);
-    RecurrenceOutputs r{ops_->createRaw(input->shape), ops_->createRaw(state)};
-    check(kth_gated_recurrence_forward(g, in, input->shape.data(), input->dimensions(), axis, mode_, h0, r.output->storeReference,
+    RecurrenceOutputs r{ops_->createRaw(gate->shape), ops_->createRaw(state)};
+    check(kth_gated_recurrence_forward(g, in, gate->shape.data(), gate->dimensions(), axis, mode_, h0, r.output->storeReference,
                                        r.finalState->storeReference));
     return r;
 }
@@ -823,8 +824,8 @@ inline Raw HipTensorOperations::GatedRecurrence::step(const Raw& gate, const Raw
     const uint64_t g = handleOf(gate), in = handleOf(input), h = handleOf(state);
     int axis = 0;
     stateShape(gate, input, state, &axis);
-    Raw r = ops_->createRaw(input->shape);
-    check(kth_gated_recurrence_forward(g, in, input->shape.data(), input->dimensions(), axis, mode_, h, r->storeReference, h));
+    Raw r = ops_->createRaw(gate->shape);
+    check(kth_gated_recurrence_forward(g, in, gate->shape.data(), gate->dimensions(), axis, mode_, h, r->storeReference, h));
     return r;
 }
 inline HipTensorOperations::RecurrenceGrads HipTensorOperations::GatedRecurrence::calculateGrads(

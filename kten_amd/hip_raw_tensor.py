@@ -494,10 +494,10 @@ class HipGatedRecurrence:
         self.mode = abi.KTH_GATE_SIGMOID if sigmoidGate else abi.KTH_GATE_GIVEN
 
     def _state_shape(self, gate, input, initial):
-        if gate.shape != input.shape:
+        if input is not None and gate.shape != input.shape:
             raise ValueError(f"Gate and input of a recurrence must have the same shape, got {gate.shape} and {input.shape}")
-        axis = sf.normalize_axis(input.shape, self.axis)
-        state = input.shape[:axis] + input.shape[axis + 1:] or [1]
+        axis = sf.normalize_axis(gate.shape, self.axis)
+        state = gate.shape[:axis] + gate.shape[axis + 1:] or [1]
         _require_size("The initial state of a recurrence", initial, sf.to_store_size(state))
         return axis, state
 
@@ -520,6 +520,8 @@ class HipGatedRecurrence:
         return output
 
     def calculateGrads(self, gate, input, initial, output, gradOut, gradFinal=None, gateRequiresGrad=True, inRequiresGrad=True, initialRequiresGrad=True):
+        """`input`, `initial` and `output` are read for the gate's gradient only, `input` only with `sigmoidGate`: None where they
+        are not."""
         if not (gateRequiresGrad or inRequiresGrad or initialRequiresGrad):
             return None, None, None
         gate._require_live(); gradOut._require_live()

@@ -1536,7 +1536,7 @@ class GatedRecurrenceFunction(SequenceLayerFunction):
         self._dropFinal()
         self.ops.markSurviveGC(final)         # as long as this function is there, whatever scopes close meanwhile
         self._final = final
-        self.saveOperands(gate, input, initial, output)
+        self.saveOperands(gate, input if self.sigmoidGate else None, initial, output)
         self.output = output
 
     @property
