@@ -385,7 +385,9 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
 #pragma unroll
     for (int k = 0; k < L; k++)                              // a step behind the last one leaves the state as it is
         if (t0 + k >= pl.steps) { v[k] = SIGMOID ? INFINITY : 1.0f; u[k] = 0.0f; }
-    const double start = w.tile == 0 && initial ? static_cast<double>(initial[w.first_state]) : 0.0;
+    double start = w.tile == 0 && initial ? static_cast<double>(initial[w.first_state]) : 0.0;
+    // final_state may be the same store: every wave's load has arrived before the barrier behind which another may write it
+    asm volatile("" : "+v"(start));
     double H = 0.0;
     Product<SIGMOID> product;
 #pragma unroll

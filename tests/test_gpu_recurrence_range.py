@@ -113,3 +113,17 @@ def test_sigmoid_gates_that_forget(outer, steps, inner, gc):
             ref.assert_within(got, want, bound, "states")
         else:
             assert (got == np.inf).all()
+
+
+@pytest.mark.parametrize("outer, steps, inner", [(8, 60, 64), (64, 250, 1024), (3, 600, 65), (1, 5000, 64), (40, 100, 20), (500, 200, 1), (2, 9000, 3)], ids=lambda v: str(v))
+def test_state_in_place_where_several_waves_read_it(outer, steps, inner, gc):
+    """The last step's state is written over the first while the waves of the sequence's first tile may still be at work."""
+    rng = np.random.default_rng(steps)
+    gate, x = (gc.createRaw([outer, steps, inner], rng.standard_normal((outer, steps, inner)).astype(np.float32)) for _ in range(2))
+    state = gc.createRaw([outer, inner], rng.standard_normal((outer, inner)).astype(np.float32))
+    apart = state.copy()
+    op = gc.gatedRecurrence(1)
+    for _ in range(10):
+        out, apart = op.calculateOutput(gate, x, apart)
+        assert_bits_equal(op.step(gate, x, state).toArray(), out.toArray(), "states")
+        assert_bits_equal(state.toArray(), apart.toArray(), "the state in place")
