@@ -163,6 +163,9 @@ def prepare(case, seed):
 # ---------------------------------------------------------------- one pass
 
 def run(state):
+    """The plain form runs on torch's stream. With `own` the calls are queued on the library's, as a program of such calls has
+    them: whoever reads the results outside the library, or stops a clock, first waits for the device (torch.cuda.synchronize,
+    or the library's sync)."""
     if own:
         return _run_own(state)
     return {"norm": _norm, "dropout": _dropout, "recurrence": _recurrence}[state.case["op"]](state)
