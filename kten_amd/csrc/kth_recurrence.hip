@@ -29,8 +29,8 @@ struct ScanShape {
     FastDiv  inner_div;
 };
 
-// exp(-|g|) to 2 u (u = 2^-24), results below the normal range included: 2^(f + n) with f the fraction of |g| log2(e), in
-// two products, by the hardware's exponential.
+// exp(-|g|) to 2 u (u = 2^-24), results below the normal range included: 2^(f + n) with f the fraction of |g| log2(e), by the
+// hardware's exponential. The product with log2(e) is made in two: by the float next to it, and by what that leaves of it.
 __device__ __forceinline__ float exp_minus_abs(float g) {
     float x = -fabsf(g);
     x = x < -110.0f ? -110.0f : x;                           // (gives 0: below half the smallest float; NaN stays NaN)
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 
 // ---------------------------------------------------------------- long sequences: tiles of steps
 
-// The scan is cut into tiles that pass a state on. A workgroup takes one tile: cw x 64 adjacent channels of one outer index
+// The scan is cut into tiles that pass a state on. A workgroup takes one tile: 64 adjacent channels of one outer index
 // (a lane per channel) and tw x L successive steps, L to a wave, which the wave keeps in registers, so that every operand
 // is read once. A step is the map K -> a K + u of the state, so a run of steps is one pair (A, H): waves exchange theirs
 // through LDS, tiles through memory.
@@ -249,8 +249,8 @@ struct TilePlan {
     uint32_t steps, inner;
     uint32_t col_blocks, groups;     // workgroups across one outer index; across all channels (outer x col_blocks)
     uint32_t tiles;                  // along the steps
-    uint32_t cw, tw;                 // waves of a workgroup across channels and along steps
-    uint32_t padded;                 // groups x cw x 64: channels with their padding
+    uint32_t tw;                     // waves of a workgroup, along the steps
+    uint32_t padded;                 // groups x 64: channels with their padding
     Wait     wait;                   // with this launch's tag
     uint32_t* tickets;               // this launch's counter
     uint64_t* pairs;                 // [tiles][padded][2]
@@ -263,7 +263,7 @@ struct TilePlan {
 
 // Where a workgroup and its waves stand.
 struct TilePlace {
-    uint32_t tile, group, lane, cwi, twi;
+    uint32_t tile, group, lane, twi;
     uint32_t channel;                // in its outer index
     uint32_t slot;                   // among the padded channels
     uint64_t base;                   // of the outer index's first step
@@ -277,31 +277,28 @@ __device__ __forceinline__ TilePlace place_tile(const TilePlan& pl, uint32_t* ld
     if (threadIdx.x == 0) *lds_ticket = pl.tiles > 1 ? atomicAdd(pl.tickets, 1u) : blockIdx.x;
     __syncthreads();
     const uint32_t ticket = __builtin_amdgcn_readfirstlane(*lds_ticket);
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    w.twi = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     w.lane = threadIdx.x & 63;
     w.tile = divide(ticket, pl.group_div);
     w.group = ticket - w.tile * pl.groups;
-    w.twi = wave / pl.cw;
-    w.cwi = wave - w.twi * pl.cw;
     const uint32_t o = divide(w.group, pl.col_div);
-    const uint32_t c = ((w.group - o * pl.col_blocks) * pl.cw + w.cwi) * 64 + w.lane;
+    const uint32_t c = (w.group - o * pl.col_blocks) * 64 + w.lane;
     w.valid = c < pl.inner;
     w.channel = w.valid ? c : pl.inner - 1;          // (a padding lane reads the last channel and writes nothing)
-    w.slot = (w.group * pl.cw + w.cwi) * 64 + w.lane;
+    w.slot = w.group * 64 + w.lane;
     w.base = static_cast<uint64_t>(o) * pl.steps * pl.inner;
     w.first_state = o * pl.inner + w.channel;
     return w;
 }
 
 // The state before this tile, from the pairs of its waves' steps and whether they are `tame`; `initial` is the state before
-// the first tile. lds: pairs of the waves, [tw][cw * 64], then of the tiles before, as many again; wild: 0 before the last
+// the first tile. lds: pairs of the waves, [tw][64], then of the tiles before, as many again; wild: 0 before the last
 // barrier. in_turn: a run of this tile is to be walked, so all are, one wave after another.
 template <bool SIGMOID>
 __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const TilePlace& w, const Pair& mine, bool tame, double initial, Pair* lds, uint32_t* wild,
                                                     bool& in_turn) {
-    const uint32_t width = pl.cw * 64, at = w.cwi * 64 + w.lane;
-    Pair* before = lds + pl.tw * width;
-    lds[w.twi * width + at] = mine;
+    Pair* before = lds + pl.tw * 64;
+    lds[w.twi * 64 + w.lane] = mine;
     if (!SIGMOID && !tame) *wild = 1;
     __syncthreads();
     in_turn = !SIGMOID && __builtin_amdgcn_readfirstlane(*wild) != 0;
@@ -309,8 +306,8 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
     const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
     if (pl.tiles > 1) {
         if (w.twi == pl.tw - 1 && w.tile + 1 < pl.tiles && many + 1 < kSuper && !in_turn) {
-            Pair total = lds[at];
-            for (uint32_t i = 1; i < pl.tw; i++) total = after<SIGMOID>(lds[i * width + at], total);
+            Pair total = lds[w.lane];
+            for (uint32_t i = 1; i < pl.tw; i++) total = after<SIGMOID>(lds[i * 64 + w.lane], total);
             if (w.tile == 0) total = Pair{0.0, advance<SIGMOID>(total, initial)};     // nobody else reads `initial`
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
             publish(word, total.A, pl.wait.tag);
@@ -326,10 +323,10 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
                 const double a = await(word, pl.wait), h = await(word + 1, pl.wait);
                 p = after<SIGMOID>(Pair{a, h}, p);
             }
-            before[w.twi * width + at] = p;
+            before[w.twi * 64 + w.lane] = p;
             state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.wait);
             __syncthreads();
-            for (uint32_t i = 0; i < pl.tw; i++) state = advance<SIGMOID>(before[i * width + at], state);
+            for (uint32_t i = 0; i < pl.tw; i++) state = advance<SIGMOID>(before[i * 64 + w.lane], state);
         }
     }
     return state;
@@ -337,13 +334,12 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
 // The state before this wave's first step from that before the tile, where the waves' pairs are composed.
 template <bool SIGMOID>
 __device__ __forceinline__ double state_before_wave(const TilePlan& pl, const TilePlace& w, double state, const Pair* lds) {
-    const uint32_t width = pl.cw * 64, at = w.cwi * 64 + w.lane;
     if (w.twi == pl.tw - 1 && w.tile % kSuper + 1 == kSuper && w.tile + 1 < pl.tiles) {
         double end = state;
-        for (uint32_t i = 0; i < pl.tw; i++) end = advance<SIGMOID>(lds[i * width + at], end);
+        for (uint32_t i = 0; i < pl.tw; i++) end = advance<SIGMOID>(lds[i * 64 + w.lane], end);
         publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.wait.tag);
     }
-    for (uint32_t i = 0; i < w.twi; i++) state = advance<SIGMOID>(lds[i * width + at], state);
+    for (uint32_t i = 0; i < w.twi; i++) state = advance<SIGMOID>(lds[i * 64 + w.lane], state);
     return state;
 }
 // What the last wave of a tile whose waves took turns hands on.
@@ -407,13 +403,12 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
     bool in_turn;
     double h = state_before_tile<SIGMOID>(pl, w, mine, product.tame(), start, lds, &wild, in_turn);
     if (in_turn) {
-        Pair* slot = lds + w.cwi * 64 + w.lane;              // wave i's of this channel: slot[i * width]; H: the state behind it
-        const uint32_t width = pl.cw * 64;
+        Pair* slot = lds + w.lane;                           // wave i's of this channel: slot[i * 64]; H: the state behind it
         double end = h;
         const double before_tile = h;
         for (uint32_t i = 0; i < pl.tw; i++) {
             if (i == w.twi) {
-                if (i > 0) h = slot[(i - 1) * width].H;
+                if (i > 0) h = slot[(i - 1) * 64].H;
                 end = h;
 #pragma unroll
                 for (int k = 0; k < L; k++) { forget(v[k]); forget(u[k]); }
@@ -422,7 +417,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_forward_tiles_kern
                     end = fma(gate_a<SIGMOID>(v[k]), end, static_cast<double>(u[k]));
                     KTH_STEPS_APART(k);
                 }
-                slot[i * width].H = end;
+                slot[i * 64].H = end;
             }
             __syncthreads();
         }
@@ -498,13 +493,12 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
     bool in_turn;
     double K = state_before_tile<SIGMOID>(pl, w, mine, product.tame(), start, lds, &wild, in_turn);
     if (in_turn) {
-        Pair* slot = lds + w.cwi * 64 + w.lane;              // wave i's of this channel: slot[i * width]; H: the state behind it
-        const uint32_t width = pl.cw * 64;
+        Pair* slot = lds + w.lane;                           // wave i's of this channel: slot[i * 64]; H: the state behind it
         double end = K;
         const double before_tile = K;
         for (uint32_t i = 0; i < pl.tw; i++) {
             if (i == w.twi) {
-                if (i > 0) K = slot[(i - 1) * width].H;
+                if (i > 0) K = slot[(i - 1) * 64].H;
                 end = K;
 #pragma unroll
                 for (int k = 0; k < L; k++) { forget(v[k]); forget(g[k]); }
@@ -513,7 +507,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
                     end = gate_a<SIGMOID>(v[k]) * (static_cast<double>(g[k]) + end);
                     KTH_STEPS_APART(k);
                 }
-                slot[i * width].H = end;
+                slot[i * 64].H = end;
             }
             __syncthreads();
         }
@@ -545,8 +539,8 @@ __global__ __launch_bounds__(kTileThreads, 4) void recurrence_backward_tiles_ker
 // takes a stretch of up to 4096 floats as memory has them, through LDS, and a thread kSub steps of one channel: thread
 // (row, j, channel), j counting the kSub-step pieces of a row. Rows that fit are taken several at a time; longer ones are
 // cut into tiles that hand a state on as above. A piece's place in LDS is padded by one float, so that the threads of a
-// wave, a piece apart, do not meet in a bank. [100000,64,1] 38 us forward (2.0 TB/s) and 87 backward, bound by the LDS and the
-// barriers of the scan over the pieces.
+// wave, a piece apart, do not meet in a bank. [100000,64,1] 38 us forward (2.0 TB/s) and 87 backward (1.8 TB/s), bound by the
+// LDS and the barriers of the scan over the pieces.
 constexpr uint32_t kNarrowThreads = 256, kSub = 16, kNarrowInner = 32;     // (inner is below kNarrowInner)
 constexpr uint32_t kNarrowFloats = kNarrowThreads * (kSub + 1);
 
@@ -847,9 +841,15 @@ __global__ __launch_bounds__(kNarrowThreads) void recurrence_backward_narrow_ker
 // Which kernel takes a call. Times in us, sigmoid gates, walk / tiles / narrow:
 //   few steps: [64,8,1024] 3.9 / 5.9 forward and 5.9 / 6.3 backward, [64,16,1024] 4.7 / 6.6 and 11.4 / 9.2,
 //     [64,32,1024] 8.5 / 9.0 and 19.8 / 12.1; [1000,8,3] 4.1 / 5.6 / 7.0 and 6.0 / 5.5 / 12.5;
-//   many channels, few side by side: [20000,32,8] 13 / 53 / 30 and 44 / 88 / 74, [100000,20,24] forward 126 / - / 311;
-//   hardly any side by side: [100000,64,1] 85 / 421 / 38 and 354 / 735 / 101, [1,66000,2] 4419 / - / 13;
-//   otherwise [1000,100,20] 18 / 14 / 21 and 61 / 21 / 34, [100,100,5] 18 / 6 / 10 and 44 / 7.5 / 15.
+//   8 to 31 side by side, many channels: [16384,200,8] 78 / 301 / 165 and 233 / 615 / 286, [8192,200,16] 68 / 162 / 159 and
+//     238 / 321 / 283, [8456,40,31] 32 / 50 / 75 and 99 / 72 / 127, [100000,20,24] forward 126 / - / 311;
+//     few channels: [512,2000,8] 371 / 103 / 69 and 1554 / 181 / 107, [256,2000,16] 368 / 62 / 67 and 1782 / 103 / 105,
+//     [132,200,31] 32 / 9 / 16 and 121 / 15 / 24, [1000,100,20] 18 / 14 / 21 and 61 / 21 / 34. Between, the border of 2^17 channels
+//     is not where the times cross, which depends on how many lie side by side: below it [2048,200,8] takes 33 / 44 / 26 and
+//     127 / 84 / 46, [8192,200,8] 48 / 154 / 90 and 172 / 310 / 154, [4096,200,16] 47 / 87 / 86 and 193 / 167 / 152,
+//     [2114,200,31] 49 / 56 / 104 and 197 / 102 / 162;
+//   hardly any side by side: [100000,64,1] 85 / 421 / 38 and 354 / 735 / 87, [1,66000,2] 4419 / - / 14; few of them: [100,100,5]
+//     18 / 6 / 10 and 44 / 7.5 / 15.
 enum class Path { walk, tiles, narrow };
 Path path_of(const ScanShape& sh, bool forward) {
     const uint32_t few = forward && sh.inner >= 8 ? 32 : 8;
@@ -883,11 +883,11 @@ int take_words(const char* what, uint64_t words, Wait* wait, uint32_t** counter,
 int plan_tiles(const char* what, const ScanShape& sh, int L, TilePlan* out) {
     TilePlan pl{};
     pl.steps = sh.steps; pl.inner = sh.inner;
-    pl.cw = 1; pl.tw = std::min<uint32_t>(kTileThreads / 64, (sh.steps + L - 1) / L);
-    pl.col_blocks = (sh.inner + pl.cw * 64 - 1) / (pl.cw * 64);
+    pl.tw = std::min<uint32_t>(kTileThreads / 64, (sh.steps + L - 1) / L);
+    pl.col_blocks = (sh.inner + 63) / 64;
     pl.groups = sh.outer * pl.col_blocks;
     pl.tiles = (sh.steps + pl.tw * L - 1) / (pl.tw * L);
-    pl.padded = pl.groups * pl.cw * 64;
+    pl.padded = pl.groups * 64;
     pl.group_div = make_div(pl.groups);
     pl.col_div = make_div(pl.col_blocks);
     if (pl.tiles > 1) {
@@ -924,7 +924,7 @@ int plan_narrow(const char* what, const ScanShape& sh, NarrowPlan* out, uint32_t
     return KTH_OK;
 }
 
-uint32_t tile_lds(const TilePlan& pl) { return 2 * pl.tw * pl.cw * 64 * static_cast<uint32_t>(sizeof(Pair)); }
+uint32_t tile_lds(const TilePlan& pl) { return 2 * pl.tw * 64 * static_cast<uint32_t>(sizeof(Pair)); }
 
 int shape_of(const char* what, const int32_t* shape, int dims, int axis, int mode, ScanShape* sh, uint64_t* n) {
     if (mode != KTH_GATE_GIVEN && mode != KTH_GATE_SIGMOID) return fail(KTH_E_ARGUMENT, "%s: gate mode %d", what, mode);
@@ -988,7 +988,7 @@ int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shap
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
         overwrite_results(ops, 5);
         LaunchScope scope("recurrence_forward_tiles_kernel", sigmoid ? "sigmoid" : "given", (3 * n + 2 * sh.channels) * 4);
-        const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
+        const dim3 grid(pl.tiles * pl.groups), block(pl.tw * 64);
         const bool lines = sh.inner % 32 == 0;
         auto* kernel = sigmoid ? (lines ? recurrence_forward_tiles_kernel<true, true, L> : recurrence_forward_tiles_kernel<true, false, L>)
                                : (lines ? recurrence_forward_tiles_kernel<false, true, L> : recurrence_forward_tiles_kernel<false, false, L>);
@@ -1043,7 +1043,7 @@ int kth_gated_recurrence_backward(uint64_t gate, uint64_t in, const int32_t* sha
         if (int rc = plan_tiles(what, sh, L, &pl)) return rc;
         overwrite_results(ops, 9);
         LaunchScope scope("recurrence_backward_tiles_kernel", sigmoid ? "sigmoid" : "given", (sigmoid ? 6 : 5) * n * 4);
-        const dim3 grid(pl.tiles * pl.groups), block(pl.cw * pl.tw * 64);
+        const dim3 grid(pl.tiles * pl.groups), block(pl.tw * 64);
         const bool lines = sh.inner % 32 == 0;
         auto* kernel = sigmoid ? (lines ? recurrence_backward_tiles_kernel<true, true, L> : recurrence_backward_tiles_kernel<true, false, L>)
                                : (lines ? recurrence_backward_tiles_kernel<false, true, L> : recurrence_backward_tiles_kernel<false, false, L>);
