@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 // launch's number: no fence, no flag, no clearing between launches (the words are cleared when the number starts again).
 // What the doubles lose is 2^-41 of themselves a tile.
 //
-// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 90 (4.5), backward 146 (4.6), [5,1999,1001] sigmoid
+// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 89 (4.5), backward 143 (4.7), [5,1999,1001] sigmoid
 // backward 69 (3.5; odd rows share cache lines with their neighbours). What bounds it is a tile's life, loads, the wait for
 // the state, stores, with two tiles in a compute unit's registers: the vector ALU is 40 % busy, and without the hand-over (its results
 // would be wrong) the same four take 46, 79, 122 and 68. Longer runs of steps spill, shorter ones have more tiles to hand over.
@@ -203,6 +203,38 @@ __device__ __forceinline__ Pair after(const Pair& later, const Pair& earlier) {
     const bool lost = SIGMOID ? fabs(A) < kLeast : fabs(A) < kLeast || fabs(later.A) <= kLeast || fabs(earlier.A) <= kLeast;
     if (lost && later.A != 0.0 && earlier.A != 0.0 && (SIGMOID || fabs(A) < INFINITY)) A = copysign(kLeast, A);
     return Pair{A, advance<SIGMOID>(later, earlier.H)};
+}
+// The state after `count` runs, their pairs `apart` from one another; and such runs as one. With given gates the chain is first
+// made without the looks that `advance` and `after` take on the way at what is lost, infinite or NaN: an infinity on the way shows
+// in the end, and the least magnitude of the products tells the rest (together 2 % of [1,65536,512]).
+template <bool SIGMOID>
+__device__ __forceinline__ double through(const Pair* pairs, uint32_t apart, uint32_t count, double state) {
+    if (!SIGMOID) {
+        double s = state;
+        for (uint32_t i = 0; i < count; i++) {
+            const Pair p = pairs[i * apart];
+            s = fma(fabs(p.A) <= kLeast ? 0.0 : p.A, s, p.H);
+        }
+        if (!__any(!(fabs(s) < INFINITY))) return s;
+    }
+    for (uint32_t i = 0; i < count; i++) state = advance<SIGMOID>(pairs[i * apart], state);
+    return state;
+}
+template <bool SIGMOID>
+__device__ __forceinline__ Pair together(const Pair* pairs, uint32_t apart, uint32_t count) {
+    Pair total = pairs[0];
+    if (!SIGMOID) {
+        double least = fabs(total.A);
+        for (uint32_t i = 1; i < count; i++) {
+            const Pair p = pairs[i * apart];
+            total = Pair{p.A * total.A, fma(p.A, total.H, p.H)};
+            least = fmin(least, fmin(fabs(p.A), fabs(total.A)));
+        }
+        if (!__any(!(least > kLeast && fabs(total.H) < INFINITY))) return total;
+        total = pairs[0];
+    }
+    for (uint32_t i = 1; i < count; i++) total = after<SIGMOID>(pairs[i * apart], total);
+    return total;
 }
 // A run after which the state is known to be `end`, whatever came before; `state` is what did (an infinite one stays infinite or
 // becomes NaN).
@@ -306,8 +338,7 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
     const uint32_t super = w.tile / kSuper, first = super * kSuper, many = w.tile - first;
     if (pl.tiles > 1) {
         if (w.twi == pl.tw - 1 && w.tile + 1 < pl.tiles && many + 1 < kSuper && !in_turn) {
-            Pair total = lds[w.lane];
-            for (uint32_t i = 1; i < pl.tw; i++) total = after<SIGMOID>(lds[i * 64 + w.lane], total);
+            Pair total = together<SIGMOID>(lds + w.lane, 64, pl.tw);
             if (w.tile == 0) total = Pair{0.0, advance<SIGMOID>(total, initial)};     // nobody else reads `initial`
             uint64_t* word = pl.pairs + (static_cast<uint64_t>(w.tile) * pl.padded + w.slot) * 2;
             publish(word, total.A, pl.wait.tag);
@@ -326,7 +357,7 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
             before[w.twi * 64 + w.lane] = p;
             state = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.padded + w.slot, pl.wait);
             __syncthreads();
-            for (uint32_t i = 0; i < pl.tw; i++) state = advance<SIGMOID>(before[i * 64 + w.lane], state);
+            state = through<SIGMOID>(before + w.lane, 64, pl.tw, state);
         }
     }
     return state;
@@ -335,12 +366,10 @@ __device__ __forceinline__ double state_before_tile(const TilePlan& pl, const Ti
 template <bool SIGMOID>
 __device__ __forceinline__ double state_before_wave(const TilePlan& pl, const TilePlace& w, double state, const Pair* lds) {
     if (w.twi == pl.tw - 1 && w.tile % kSuper + 1 == kSuper && w.tile + 1 < pl.tiles) {
-        double end = state;
-        for (uint32_t i = 0; i < pl.tw; i++) end = advance<SIGMOID>(lds[i * 64 + w.lane], end);
+        const double end = through<SIGMOID>(lds + w.lane, 64, pl.tw, state);
         publish(pl.states + static_cast<uint64_t>(w.tile / kSuper) * pl.padded + w.slot, end, pl.wait.tag);
     }
-    for (uint32_t i = 0; i < w.twi; i++) state = advance<SIGMOID>(lds[i * 64 + w.lane], state);
-    return state;
+    return through<SIGMOID>(lds + w.lane, 64, w.twi, state);
 }
 // What the last wave of a tile whose waves took turns hands on.
 __device__ __forceinline__ void hand_on_end(const TilePlan& pl, const TilePlace& w, double before_tile, double end) {
@@ -644,7 +673,7 @@ __device__ __forceinline__ double narrow_state_before(const NarrowPlan& pl, cons
             if (threadIdx.x < pl.inner) {
                 const uint32_t channel = w.o0 * pl.inner + threadIdx.x;
                 double s = super == 0 ? 0.0 : await(pl.states + static_cast<uint64_t>(super - 1) * pl.channels + channel, pl.wait);
-                for (uint32_t t = 0; t < many; t++) s = advance<SIGMOID>(handed[t * pl.inner + threadIdx.x], s);
+                s = through<SIGMOID>(handed + threadIdx.x, pl.inner, many, s);
                 carried[threadIdx.x] = s;
                 if (many + 1 == kSuper && w.tile + 1 < pl.tiles && !in_turn)
                     publish(pl.states + static_cast<uint64_t>(super) * pl.channels + channel, advance<SIGMOID>(total[threadIdx.x], s), pl.wait.tag);
