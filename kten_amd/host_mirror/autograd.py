@@ -197,6 +197,8 @@ class AGTensor(Tensor):
     def dropout(self, p, generator, training=True, residual=None):
         """[residual +] dropout(this) with the next numbers of `generator`; outside training [residual +] this."""
         if not training:
+            if residual is not None:
+                _require_residual(self.shape, residual.shape)
             return self if residual is None else residual + self
         return DropoutFunction(p, generator, self.ops)(self, residual)
 
@@ -1488,6 +1490,11 @@ class CounterGenerator:
         return first
 
 
+def _require_residual(shape, residual):
+    if list(residual) != list(shape):
+        raise ValueError(f"The residual of a dropout must have its input's shape {list(shape)}, got {residual}")
+
+
 class DropoutFunction(SequenceLayerFunction):
     """Dropout with the numbers of a CounterGenerator, plus a residual of the same shape if one is given. Nothing is saved."""
 
@@ -1497,8 +1504,8 @@ class DropoutFunction(SequenceLayerFunction):
 
     def __call__(self, input, residual):
         super().__call__(input, residual)
-        if residual is not None and list(self.operands[1].shape) != self.cachedShape:
-            raise ValueError(f"The residual of a dropout must have its input's shape {self.cachedShape}, got {self.operands[1].shape}")
+        if residual is not None:
+            _require_residual(self.cachedShape, self.operands[1].shape)
         self.dropoutOp = self.ops.dropout(self.p, self.generator.seed, self.generator.offset)
         self.generator.reserve(sf.to_store_size(self.cachedShape))
         return self
