@@ -372,8 +372,10 @@ int kth_batch_norm_backward(uint64_t in, const int32_t* shape, int dims, int axi
 
 /* The operators of a residual block over sequences. The reference has none of them (its layers stop at batch
  * normalisation); their operands follow kth_batch_norm_*: dense tensors of `shape`, `axis` already normalised, 0 for an
- * operand that is not given or a result that is not required, sums and states in f64 inside. Deterministic. A result
- * may share its store with another operand only where that is said. */
+ * operand that is not given or a result that is not required. Sums, statistics and states are f64 inside; a sigmoid gate and
+ * what it leaves of the input are floats first, partial sums of the weights' gradients are f64 sums rounded to float once, and a
+ * state that long sequences hand on between their tiles keeps 41 bits. Deterministic. A result may share its store with
+ * another operand only where that is said. A call that is refused, for want of memory too, leaves its results as they were. */
 
 /* Layer normalisation over the dims axis .. dims-1 (cols = their product, rows = that of the dims before):
  * out = (in - mean) / sqrt(var + epsilon) * gamma + beta per row, var the mean squared deviation. gamma and beta hold
@@ -403,10 +405,11 @@ int kth_dropout(uint64_t in, uint64_t n, double p, uint64_t seed, uint64_t offse
  * is 0. One step at a time (shape[axis] == 1, initial and final_state the same store, which is then updated in place) is
  * the form for single tokens. An infinite gate (KTH_GATE_GIVEN) leaves its channel infinite or NaN from its step on. Given
  * gates may decay and grow as they like: a state that falls below the range of a double is 0 from there on and one that
- * grows past it infinite or NaN, as step by step; one that falls by more than 2^1022 within a few hundred steps
- * counts as 0 already. Long sequences are cut into tiles that wait for one another inside the launch; should such a wait be given up (after seconds,
- * on a device that stands still), the results behind it are NaN and the next kth_sync, kth_download, kth_read_scalar or
- * kth_contains_nan returns KTH_E_DEVICE, once. */
+ * grows past it infinite or NaN, as step by step; one that falls by more than 2^1022 within a few hundred steps (a few
+ * thousand with fewer than 8 channels side by side) counts as 0 already. Long sequences are cut into tiles that wait for
+ * one another inside the launch; should such a wait be given up (after seconds, on a device that stands still), the
+ * results behind it are NaN and the next kth_sync, kth_download, kth_read_scalar or kth_contains_nan returns
+ * KTH_E_DEVICE, once. */
 int kth_gated_recurrence_forward(uint64_t gate, uint64_t in, const int32_t* shape, int dims, int axis, int mode, uint64_t initial,
                                  uint64_t out, uint64_t final_state);
 
