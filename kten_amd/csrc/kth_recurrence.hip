@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_backward_kernel(const float
 // launch's number: no fence, no flag, no clearing between launches (the words are cleared when the number starts again).
 // What the doubles lose is 2^-41 of themselves a tile.
 //
-// [8,2048,1024] sigmoid forward 47 us (4.3 TB/s), [1,65536,512] given forward 89 (4.5), backward 143 (4.7), [5,1999,1001] sigmoid
+// [8,2048,1024] sigmoid forward 48 us (4.2 TB/s), [1,65536,512] given forward 89 (4.5), backward 143 (4.7), [5,1999,1001] sigmoid
 // backward 69 (3.5; odd rows share cache lines with their neighbours). What bounds it is a tile's life, loads, the wait for
 // the state, stores, with two tiles in a compute unit's registers: the vector ALU is 40 % busy, and without the hand-over (its results
 // would be wrong) the same four take 46, 79, 122 and 68. Longer runs of steps spill, shorter ones have more tiles to hand over.
